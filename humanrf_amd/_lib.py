@@ -36,6 +36,13 @@ class AdamTensor(ctypes.Structure):
                 ("group", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class AdamWTensor(ctypes.Structure):
+    """hrf_adamw_tensor (include/hrf.h)."""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("copy", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("base", ctypes.c_int64), ("first_tile", ctypes.c_int32), ("kind", ctypes.c_int32),
+                ("lr_scale", ctypes.c_double), ("decay_scale", ctypes.c_double)]
+
+
 class GradScaler(ctypes.Structure):
     """hrf_grad_scaler (include/hrf.h)."""
     _fields_ = [("scale", ctypes.c_float), ("growth_factor", ctypes.c_float), ("backoff_factor", ctypes.c_float),
@@ -52,7 +59,7 @@ def build(force: bool = False) -> str:
     return LIB_PATH
 
 
-_VP, _I64, _I32, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_VP, _I64, _I32, _F, _D = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_double
 
 _SIGNATURES = {
     "hrf_abi_version": [],
@@ -98,6 +105,8 @@ _SIGNATURES = {
     "hrf_render_loss_fused": [_VP] * 6 + [_I64, _I64, _F, _F, _F, _F] + [_VP] * 9 + [_VP],
     "hrf_adam_step": [_VP] * 5 + [_I64] + [_F] * 7 + [_VP, _VP],
     "hrf_adam_multi": [_VP, _I32, _I32, _I64] + [_F] * 5 + [_VP, _VP, _VP, _VP],
+    "hrf_adamw_multi": [_VP, _VP, _I32, _I32, _I32] + [_VP] * 5 + [_D, _VP] + [_D] * 6 + [_VP] * 3 + [ctypes.c_uint32, _I32, _VP],
+    "hrf_grad_norm_multi": [_VP, _VP, _I32, _D] + [_VP] * 5,
     "hrf_uniform_fill": [ctypes.c_uint32, _I64, _VP, _VP],
     "hrf_weights_fwd": [_VP] * 4 + [_I64, _VP, _VP],
     "hrf_weights_bwd": [_VP] * 5 + [_I64, _VP, _VP],
@@ -120,6 +129,8 @@ def lib() -> ctypes.CDLL:
             l.hrf_last_error.restype = ctypes.c_char_p
             l.hrf_adam_workspace_bytes.restype = ctypes.c_size_t
             l.hrf_adam_workspace_bytes.argtypes = []
+            l.hrf_adamw_workspace_bytes.restype = ctypes.c_size_t
+            l.hrf_adamw_workspace_bytes.argtypes = []
             l.hrf_scatter_workspace_bytes.restype = ctypes.c_size_t
             l.hrf_scatter_workspace_bytes.argtypes = [_I64, _I32]
             l.hrf_scatter_signals_per_segment.restype = ctypes.c_int64
@@ -138,7 +149,7 @@ def lib() -> ctypes.CDLL:
 
 def exported_symbols():
     """Names hrf.h declares (used by the CPU-side ABI test)."""
-    return ["hrf_last_error", "hrf_adam_workspace_bytes", "hrf_scatter_workspace_bytes", "hrf_scatter_signals_per_segment",
+    return ["hrf_last_error", "hrf_adam_workspace_bytes", "hrf_adamw_workspace_bytes", "hrf_scatter_workspace_bytes", "hrf_scatter_signals_per_segment",
             "hrf_can_stream_wait_value"] + list(_SIGNATURES.keys())
 
 

@@ -605,6 +605,201 @@ def adam_multi(descriptors: torch.Tensor, count: int, num_groups: int, max_eleme
                                         grad_scale, ptr(state), ptr(scaler), ptr(workspace), stream_ptr()))
 
 
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOGUARD = _NoGuard()
+
+
+def _on_device(device: torch.device):
+    """Context in which `device` is the current one (a launch goes to the current device, on ITS current stream)."""
+    return _NOGUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_ADAMW_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class AdamWPlan:
+    """The tensors of an AdamW step (ops.adamw_multi) and their optimizer state, built once and kept from step to step.
+
+    params: fp32, fp16 or bf16 tensors of one GPU, contiguous, of any length; a 16-bit parameter has no fp32 master, each step rounds it
+        to the nearest value of its type. grads: their gradients (fp32, fp16 or bf16, the same lengths; None entries are not stepped and
+        keep their step count), at addresses that stay; `set_grads` gives others. copies: 16-bit copies of fp32 parameters that the step
+        refreshes (None entries: none).
+    state_bits: 32 = fp32 moments; 8 = e4m3 codes of the first moment and of the square root of the second, one fp32 scale per 256 values.
+    state: flat buffers to take over (`state` of another plan over tensors of the same lengths); zeros otherwise. step: steps taken.
+    seed: of the random rounding of 8-bit states. lr_scales, decay_scales: factors of lr and weight_decay per tensor (default 1).
+
+    `state` holds the flat buffers by name ("exp_avg", "exp_avg_sq"; with 8 bits "exp_avg", "exp_avg_scale", "exp_avg_root",
+    "exp_avg_root_scale"): tensor k's values are [offsets[k], offsets[k] + n), padded with zeros to a multiple of 256.
+    `steps` holds the step count of each tensor, on the device. One step or norm of a plan runs at a time (one stream, or ordered)."""
+
+    TILE, BLOCK = 2048, 256
+
+    def __init__(self, params, grads=None, copies=None, state_bits: int = 32, state=None, step: int = 0, seed: int = 0,
+                 lr_scales=None, decay_scales=None):
+        params = list(params)
+        if not params:
+            raise RuntimeError("AdamWPlan: no parameters")
+        if state_bits not in (8, 32):
+            raise RuntimeError(f"AdamWPlan: state_bits must be 8 or 32, got {state_bits}")
+        if int(step) < 0:
+            raise RuntimeError("AdamWPlan: negative step count")
+        for p in params:
+            _chk(p, "parameter")
+            if p.dtype not in _ADAMW_KINDS:
+                raise RuntimeError(f"AdamWPlan: parameters must be float32, float16 or bfloat16, got {p.dtype}")
+            if p.device != params[0].device:
+                raise RuntimeError("AdamWPlan: the parameters lie on several devices")
+        copies = [None] * len(params) if copies is None else list(copies)
+        if len(copies) != len(params):
+            raise RuntimeError("AdamWPlan: one copy (or None) for each parameter")
+        for p, c in zip(params, copies):
+            if c is None:
+                continue
+            _chk(c, "16-bit copy")
+            if p.dtype != torch.float32 or c.dtype not in (torch.float16, torch.bfloat16):
+                raise RuntimeError("AdamWPlan: copies are float16 or bfloat16 copies of float32 parameters")
+            if c.numel() != p.numel() or c.device != p.device:
+                raise RuntimeError("AdamWPlan: a copy has its parameter's length and device")
+        self.params, self.copies, self.state_bits, self.seed = params, copies, int(state_bits), int(seed) & 0xFFFFFFFF
+        self.device = params[0].device
+        self.lr_scales = [1.0] * len(params) if lr_scales is None else [float(x) for x in lr_scales]
+        self.decay_scales = [1.0] * len(params) if decay_scales is None else [float(x) for x in decay_scales]
+        for scales in (self.lr_scales, self.decay_scales):
+            if len(scales) != len(params) or not all(0.0 <= x < float("inf") for x in scales):
+                raise RuntimeError("AdamWPlan: one finite factor >= 0 for each parameter")
+        self.offsets, self._first_tile, tiles, at, count = [], [], [], 0, 0
+        for k, p in enumerate(params):
+            self.offsets.append(at)
+            self._first_tile.append(count)
+            here = -(-p.numel() // self.TILE)
+            tiles.append(here)
+            count += here
+            at += -(-p.numel() // self.BLOCK) * self.BLOCK
+        self.numel, self.num_tiles = at, count
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamWPlan: build the plan before the capture of a graph")
+        self.state = self._take_state(state)
+        self._ctl = torch.zeros(4 + len(params), dtype=torch.int32, device=self.device)
+        if step:
+            self._ctl[4:] = int(step)
+        self._tile_tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), torch.tensor(tiles)).to(self.device)
+        self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
+        self._desc = None
+        self.grads = None
+        self.set_grads([None] * len(params) if grads is None else grads)
+
+    def _take_state(self, state):
+        blocks = self.numel // self.BLOCK
+        want = ({"exp_avg": (torch.float32, self.numel), "exp_avg_sq": (torch.float32, self.numel)} if self.state_bits == 32 else
+                {"exp_avg": (torch.float8_e4m3fn, self.numel), "exp_avg_scale": (torch.float32, blocks),
+                 "exp_avg_root": (torch.float8_e4m3fn, self.numel), "exp_avg_root_scale": (torch.float32, blocks)})
+        if state is None:
+            return {name: torch.zeros(n, dtype=torch.uint8 if dt == torch.float8_e4m3fn else dt, device=self.device).view(dt)
+                    for name, (dt, n) in want.items()}
+        if set(state) != set(want):
+            raise RuntimeError(f"AdamWPlan: state must hold {sorted(want)}, got {sorted(state)}")
+        for name, (dt, n) in want.items():
+            _chk(state[name], name, dt)
+            if state[name].numel() != n or state[name].device != self.device:
+                raise RuntimeError(f"AdamWPlan: state {name} must have {n} values on {self.device}")
+            if state[name].data_ptr() % 16:
+                raise RuntimeError(f"AdamWPlan: state {name} must begin at a multiple of 16 bytes")
+        return {name: state[name] for name in want}
+
+    def set_grads(self, grads) -> None:
+        """Other gradient tensors (or None) for the next steps: the descriptors are written anew, on the current stream."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise RuntimeError("AdamWPlan: one gradient (or None) for each parameter")
+        for p, g in zip(self.params, grads):
+            if g is None:
+                continue
+            _chk(g, "gradient")
+            if g.dtype not in _ADAMW_KINDS:
+                raise RuntimeError(f"AdamWPlan: gradients must be float32, float16 or bfloat16, got {g.dtype}")
+            if g.numel() != p.numel() or g.device != p.device:
+                raise RuntimeError("AdamWPlan: a gradient has its parameter's length and device")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamWPlan: the gradients' addresses change inside the capture of a graph; keep them in place "
+                               "(zero them instead of dropping them) and set them before the capture")
+        arr = (_lib.AdamWTensor * len(grads))()
+        for k, (p, g, c) in enumerate(zip(self.params, grads, self.copies)):
+            kind = _ADAMW_KINDS[p.dtype] | (_ADAMW_KINDS[g.dtype] << 2 if g is not None else 0) | (_ADAMW_KINDS[c.dtype] << 4 if c is not None else 0)
+            # (an empty tensor has no storage, but it has a gradient: its step count advances)
+            arr[k] = _lib.AdamWTensor(ptr(p), None if g is None else (ptr(g) or 1), ptr(c), p.numel(), self.offsets[k], self._first_tile[k], kind,
+                                      self.lr_scales[k], self.decay_scales[k])
+        host = torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).pin_memory()
+        with _on_device(self.device):
+            if self._desc is None:
+                self._desc = torch.empty(host.numel(), dtype=torch.uint8, device=self.device)
+            self._desc.copy_(host, non_blocking=True)
+        self.grads = grads
+
+    @property
+    def steps(self) -> torch.Tensor:
+        """int32 (tensors,), on the device: steps taken by each tensor."""
+        return self._ctl[4:]
+
+    @property
+    def skipped(self) -> torch.Tensor:
+        """int32 (1,), on the device: steps skipped for gradients that were not finite."""
+        return self._ctl[1:2]
+
+
+def grad_norm_multi(plan: AdamWPlan, grad_scale: float = 1.0, scaler=None, out=None) -> torch.Tensor:
+    """2-norm of all gradients of the plan over grad_scale (and the loss scale of `scaler`), one fp32 value on the device: summed in 64 bits
+    and in a fixed order, so the same gradients give the same bits. Not finite when a gradient is not."""
+    _chk(scaler, "grad scaler", torch.uint8); _chk(out, "norm", torch.float32)
+    if out is None:
+        out = torch.empty((), dtype=torch.float32, device=plan.device)
+    elif out.numel() != 1 or out.device != plan.device:
+        raise RuntimeError("grad_norm_multi: the norm is one value on the plan's device")
+    if scaler is not None and scaler.device != plan.device:
+        raise RuntimeError("grad_norm_multi: the grad scaler lies on another device")
+    with _on_device(plan.device), _span("grad_norm", plan.numel):
+        check(_lib.lib().hrf_grad_norm_multi(ptr(plan._desc), ptr(plan._tile_tensor), plan.num_tiles, float(grad_scale), ptr(scaler),
+                                             ptr(plan._ctl), ptr(plan._ws), ptr(out), stream_ptr()))
+    return out
+
+
+def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weight_decay: float = 0.0, norm=None, max_norm=None,
+                grad_scale: float = 1.0, flags=None, scaler=None, zero_grad: bool = False) -> None:
+    """torch.optim.AdamW step of every tensor of the plan that has a gradient, in one launch (hrf_adamw_multi, include/hrf.h).
+    lr: a number, or an fp32 tensor of one value on the device (a schedule inside a captured graph). norm: what grad_norm_multi gave for
+    these gradients; a norm that is not finite skips the step, and with max_norm the gradients are scaled down to that norm. flags:
+    int32 (>= 1,), the step is skipped when flags[0] != 0. scaler: ops.grad_scaler, gradients are unscaled and its scale is updated."""
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        _chk(lr, "lr", torch.float32)
+        lr_dev, lr = lr, 0.0
+        if lr_dev.numel() != 1:
+            raise RuntimeError("adamw_multi: lr must be one value")
+    _chk(norm, "norm", torch.float32); _chk(flags, "flags", torch.int32); _chk(scaler, "grad scaler", torch.uint8)
+    for t in (lr_dev, norm, flags, scaler):
+        if t is not None and t.device != plan.device:
+            raise RuntimeError("adamw_multi: lr, norm, flags and scaler lie on the plan's device")
+        if t is not None and t.numel() < 1:
+            raise RuntimeError("adamw_multi: lr, norm, flags and scaler hold a value")
+    if max_norm is not None and (norm is None or not float(max_norm) > 0.0):
+        raise RuntimeError("adamw_multi: max_norm is a positive number and needs the norm of the gradients")
+    st = list(plan.state.values())
+    if plan.state_bits == 32:
+        st = [st[0], None, st[1], None]
+    with _on_device(plan.device), _span("adamw", plan.numel):
+        check(_lib.lib().hrf_adamw_multi(ptr(plan._desc), ptr(plan._tile_tensor), plan.num_tiles, len(plan.params), plan.state_bits,
+                                         ptr(st[0]), ptr(st[2]), ptr(st[1]), ptr(st[3]), ptr(plan._ctl), float(lr), ptr(lr_dev),
+                                         float(betas[0]), float(betas[1]), float(eps), float(weight_decay), float(grad_scale),
+                                         0.0 if max_norm is None else float(max_norm), ptr(norm), ptr(flags), ptr(scaler), plan.seed,
+                                         1 if zero_grad else 0, stream_ptr()))
+
+
 def compose_forward(xyz_f, xyt_f, yzt_f, xzt_f, vectors, xyzt):
     for a, nm in ((xyz_f, "xyz_features"), (xyt_f, "xyt_features"), (yzt_f, "yzt_features"), (xzt_f, "xzt_features")):
         _chk(a, nm, torch.float16)

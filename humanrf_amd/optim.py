@@ -1,0 +1,149 @@
+"""AdamW as an optimizer object over ops.adamw_multi: for a caller that keeps a torch training loop (the reference's own Trainer over
+HumanRF.get_params, humanrf/run.py:101, or any other model) and wants decoupled weight decay, 8-bit states or clipping by the global norm
+in one or two launches a step. TrainEngine has its own fused Adam (ops.adam_multi) and does not go through this."""
+from __future__ import annotations
+
+from typing import Dict, Optional
+
+import torch
+
+from . import ops
+
+
+class AdamW(torch.optim.Optimizer):
+    """params, lr, betas, eps, weight_decay: as torch.optim.AdamW, with the reference's betas and eps as defaults; lr and weight_decay may
+    differ between parameter groups, betas and eps may not. state_bits: 32 or 8 (ops.AdamWPlan). max_grad_norm: clip the gradients of all
+    groups together to this norm; a step whose norm is not finite is then skipped. copies: {parameter: 16-bit tensor} refreshed by the
+    step. The parameters lie on one GPU.
+
+    Gradients that stay in place from step to step (`zero_grad(set_to_none=False)`, or `step(zero_grad=True)`, which zeroes them in the
+    same pass) cost nothing on the host; new ones are written into the descriptors first. A graph of the step is captured after one eager
+    step with the gradients in place. `step` advances the parameters' version counters, so that casts of them are renewed."""
+
+    def __init__(self, params, lr=1e-2, betas=(0.9, 0.99), eps: float = 1e-15, weight_decay: float = 1e-2, state_bits: int = 32,
+                 max_grad_norm: Optional[float] = None, seed: int = 0, copies: Optional[Dict[torch.Tensor, torch.Tensor]] = None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
+            raise ValueError("max_grad_norm must be positive")
+        self._plan = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=float(eps), weight_decay=float(weight_decay)))
+        self.state_bits, self.max_grad_norm, self.seed = int(state_bits), max_grad_norm, int(seed)
+        self._copies = dict(copies) if copies else {}
+        self._key = None
+        self._hyper()
+
+    def add_param_group(self, param_group) -> None:
+        if self._plan is not None:
+            raise RuntimeError("AdamW: add parameter groups before the first step")
+        super().add_param_group(param_group)
+
+    def _all(self):
+        return [p for group in self.param_groups for p in group["params"]]
+
+    def _hyper(self):
+        """(lr, weight decay) of the call and the factors of each parameter."""
+        groups = self.param_groups
+        first = groups[0]
+        for g in groups:
+            if tuple(g["betas"]) != tuple(first["betas"]) or g["eps"] != first["eps"]:
+                raise ValueError("AdamW: betas and eps are the same in all parameter groups")
+        if any(isinstance(g["lr"], torch.Tensor) for g in groups):
+            if any(g["lr"] is not first["lr"] for g in groups):
+                raise ValueError("AdamW: an lr that is a tensor is the same tensor in all parameter groups")
+            lr, scale = first["lr"], [1.0] * len(groups)
+        else:
+            lr = max(float(g["lr"]) for g in groups)
+            scale = [float(g["lr"]) / lr if lr > 0.0 else 1.0 for g in groups]
+        decay = max(float(g["weight_decay"]) for g in groups)
+        decays = [float(g["weight_decay"]) / decay if decay > 0.0 else 1.0 for g in groups]
+        return lr, decay, [s for s, g in zip(scale, groups) for _ in g["params"]], [d for d, g in zip(decays, groups) for _ in g["params"]]
+
+    def _ensure_plan(self) -> ops.AdamWPlan:
+        if self._plan is None:
+            params = self._all()
+            self._plan = ops.AdamWPlan([p.detach() for p in params], copies=[self._copies.get(p) for p in params],
+                                       state_bits=self.state_bits, seed=self.seed)
+        return self._plan
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale: float = 1.0, flags=None, scaler=None, zero_grad: bool = False):
+        """grad_scale, flags, scaler, zero_grad: as ops.adamw_multi."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params = self._all()
+        grads = [p.grad for p in params]
+        if all(g is None for g in grads):
+            return loss
+        lr, decay, lr_scales, decay_scales = self._hyper()
+        plan = self._ensure_plan()
+        key = ([(0 if g is None else g.data_ptr(), None if g is None else g.dtype) for g in grads], [p.data_ptr() for p in params],
+               lr_scales, decay_scales)
+        if key != self._key:
+            for g in grads:
+                if g is not None and g.layout != torch.strided:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
+            plan.params, plan.lr_scales, plan.decay_scales = [p.detach() for p in params], lr_scales, decay_scales
+            for p in plan.params:
+                ops._chk(p, "parameter")
+            plan.set_grads(grads)
+            plan.grads = None            # (held by the parameters; a second reference here would keep dropped gradients alive)
+            self._key = key
+        group = self.param_groups[0]
+        norm = ops.grad_norm_multi(plan, grad_scale, scaler) if self.max_grad_norm is not None else None
+        ops.adamw_multi(plan, lr, betas=group["betas"], eps=group["eps"], weight_decay=decay, norm=norm, max_norm=self.max_grad_norm,
+                        grad_scale=grad_scale, flags=flags, scaler=scaler, zero_grad=zero_grad)
+        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+        return loss
+
+    # ------------------------------------------------------------------ checkpoints
+    def _views(self, k: int):
+        plan, n = self._plan, self._plan.params[k].numel()
+        at, size = plan.offsets[k], -(-n // plan.BLOCK) * plan.BLOCK
+        out = {}
+        for name, buf in plan.state.items():
+            if name.endswith("_scale"):
+                out[name] = buf[at // plan.BLOCK:(at + size) // plan.BLOCK]
+            else:
+                out[name] = buf[at:at + n].view(self._plan.params[k].shape)
+        return out
+
+    def state_dict(self):
+        """torch.optim.AdamW's layout: per parameter "step", "exp_avg", "exp_avg_sq" (with 8 bits "exp_avg", "exp_avg_root" and their
+        scales instead); a checkpoint with 32-bit states loads into either."""
+        sd = super().state_dict()
+        if self._plan is not None:
+            steps = self._plan.steps.cpu()
+            sd["state"] = {k: {"step": steps[k].float(), **{name: v.clone() for name, v in self._views(k).items()}}
+                           for k in range(len(self._plan.params))}
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self._hyper()
+        plan = self._ensure_plan()
+        for buf in plan.state.values():
+            buf.view(torch.uint8).zero_()
+        plan.steps.zero_()
+        for k in range(len(plan.params)):
+            entry = state_dict["state"].get(k)
+            if not entry:
+                continue
+            for name, view in self._views(k).items():
+                if name not in entry:
+                    raise RuntimeError(f"AdamW: the checkpoint has no {name} for parameter {k}: was it written with states in other bits?")
+                value = entry[name]
+                if value.shape != view.shape or (view.dtype == torch.float8_e4m3fn) != (value.dtype == torch.float8_e4m3fn):
+                    raise RuntimeError(f"AdamW: {name} of parameter {k} has another shape or type in the checkpoint")
+                if view.dtype == torch.float8_e4m3fn:
+                    view.view(torch.uint8).copy_(value.view(torch.uint8))
+                else:
+                    view.copy_(value)
+            plan.steps[k] = int(entry["step"])
+        self._key = None
+
+
+__all__ = ["AdamW"]

@@ -524,6 +524,43 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
                    float beta1, float beta2, float eps, float grad_scale, int32_t* state, hrf_grad_scaler* scaler,
                    void* workspace, hrf_stream_t stream);
 
+/* AdamW (torch.optim.AdamW: decoupled weight decay) over many tensors in one launch, moments in 32 or in 8 bits. No counterpart in
+ * the reference, whose optimizer is torch.optim.Adam on fp32 tensors (humanrf/run.py:101).
+ * tensors: DEVICE array of `count` descriptors; tile_tensor: DEVICE int32[num_tiles], the tensor of each tile of 2048 elements, the
+ * tiles of tensor k being first_tile .. first_tile + ceil(n / 2048) - 1.
+ * States lie in flat buffers, tensor k's from position `base` (a multiple of 256) on, each tensor padded with zeros to whole blocks
+ * of 256:
+ *   state_bits 32: exp_avg, second = fp32 moments m and v;
+ *   state_bits 8:  exp_avg, second = e4m3 (OCP fn) codes of m and of sqrt(v), exp_avg_scale / second_scale = fp32, one per block. Codes
+ *                  are rounded up or down at random, without bias, by a hash of (seed, step, position): the same call gives the same bits.
+ * ctl: DEVICE int32[4 + count] = { internal, steps skipped, internal, internal, steps[count] }, zero at first. The launch advances the
+ *   step counts of the tensors that have a gradient.
+ * lr: host value, or DEVICE fp32 lr_dev (may be NULL). Gradients are divided by grad_scale (times scaler->scale when a scaler is given)
+ *   and, with max_norm > 0, multiplied by min(1, max_norm / (*norm + 1e-6)). The step is skipped (steps and values stay) when
+ *   flags[0] != 0 or *norm (either may be NULL) is not finite; with a scaler its scale is then backed off, and grown as GradScaler does.
+ * zero_grad != 0: the gradients are zeroed in the same pass. eps must be a positive normal fp32 number. */
+typedef struct hrf_adamw_tensor {
+    void* param;
+    void* grad;        /* NULL: not stepped this time */
+    void* copy;        /* 16-bit copy of the parameter to refresh, or NULL */
+    int64_t n;
+    int64_t base;
+    int32_t first_tile;
+    int32_t kind;      /* bits 0-1 / 2-3 / 4-5: type of param / grad / copy, 0 = fp32, 1 = fp16, 2 = bf16 */
+    double lr_scale;   /* this tensor's learning rate is lr * lr_scale, ... */
+    double decay_scale; /* ... its weight decay weight_decay * decay_scale */
+} hrf_adamw_tensor;
+size_t hrf_adamw_workspace_bytes(void);
+int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor, int num_tiles, int count, int state_bits,
+                    void* exp_avg, void* second, float* exp_avg_scale, float* second_scale, int32_t* ctl, double lr,
+                    const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
+                    double max_norm, const float* norm, const int32_t* flags, hrf_grad_scaler* scaler, uint32_t seed, int zero_grad,
+                    hrf_stream_t stream);
+/* *out = 2-norm of all gradients of the tensors divided by grad_scale (times scaler->scale), summed in 64 bits in a fixed order.
+ * workspace: DEVICE scratch of hrf_adamw_workspace_bytes() bytes; ctl as above. One norm or step of the same ctl at a time. */
+int hrf_grad_norm_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor, int num_tiles, double grad_scale,
+                        const hrf_grad_scaler* scaler, int32_t* ctl, void* workspace, float* out, hrf_stream_t stream);
+
 /* out[i] = value i of the counter-based uniform [0,1) stream `seed` (24 random bits, like torch.rand): the numbers
  * hrf_prune_march draws in-kernel for jitter_seed == seed. n < 2^32. */
 int hrf_uniform_fill(uint32_t seed, int64_t n, float* out, hrf_stream_t stream);

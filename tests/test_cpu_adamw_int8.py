@@ -1,0 +1,90 @@
+"""What the AdamW step and the 8-bit integer product refuse, on the CPU: through the C entry points (arguments are looked at before
+anything is launched) and through the Python wrappers."""
+import ctypes
+
+import pytest
+import torch
+
+FAKE = 1 << 20      # an address that is never followed: every call below is refused before a launch
+
+
+def _adamw(lib, **change):
+    a = dict(tensors=FAKE, tile_tensor=FAKE, num_tiles=1, count=1, state_bits=32, exp_avg=FAKE, second=FAKE, exp_avg_scale=None,
+             second_scale=None, ctl=FAKE, lr=1e-2, lr_dev=None, beta1=0.9, beta2=0.99, eps=1e-15, weight_decay=0.0, grad_scale=1.0,
+             max_norm=0.0, norm=None, flags=None, scaler=None, seed=0, zero_grad=0, stream=None)
+    a.update(change)
+    return lib.hrf_adamw_multi(*a.values())
+
+
+@pytest.mark.parametrize("change,said", [
+    (dict(num_tiles=-1), b"counts"), (dict(count=-1), b"counts"), (dict(state_bits=16), b"8 or in 32"),
+    (dict(lr=-1.0), b"hyper"), (dict(lr=float("nan")), b"hyper"), (dict(beta1=1.0), b"hyper"), (dict(beta2=-0.1), b"hyper"),
+    (dict(weight_decay=float("inf")), b"hyper"), (dict(weight_decay=-1.0), b"hyper"), (dict(grad_scale=0.0), b"hyper"),
+    (dict(eps=0.0), b"eps"), (dict(eps=1e-40), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(max_norm=1.0), b"norm"),
+    (dict(tensors=None), b"NULL"), (dict(tile_tensor=None), b"NULL"), (dict(exp_avg=None), b"NULL"), (dict(second=None), b"NULL"),
+    (dict(ctl=None), b"NULL"), (dict(state_bits=8), b"scales"), (dict(state_bits=8, exp_avg_scale=FAKE), b"scales"),
+])
+def test_the_step_refuses(change, said):
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    assert _adamw(lib, **change) != 0
+    assert b"hrf_adamw_multi" in lib.hrf_last_error() and said in lib.hrf_last_error()
+
+
+def test_a_step_over_nothing_is_nothing():
+    from humanrf_amd import _lib
+    assert _adamw(_lib.lib(), num_tiles=0, tensors=None, tile_tensor=None, exp_avg=None, second=None, ctl=None) == 0
+
+
+@pytest.mark.parametrize("args", [
+    (FAKE, FAKE, -1, 1.0, None, FAKE, FAKE, FAKE, None), (FAKE, FAKE, 1, 0.0, None, FAKE, FAKE, FAKE, None),
+    (FAKE, FAKE, 1, float("nan"), None, FAKE, FAKE, FAKE, None), (None, FAKE, 1, 1.0, None, FAKE, FAKE, FAKE, None),
+    (FAKE, None, 1, 1.0, None, FAKE, FAKE, FAKE, None), (FAKE, FAKE, 1, 1.0, None, None, FAKE, FAKE, None),
+    (FAKE, FAKE, 1, 1.0, None, FAKE, None, FAKE, None), (FAKE, FAKE, 1, 1.0, None, FAKE, FAKE, None, None),
+])
+def test_the_norm_refuses(args):
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    assert lib.hrf_grad_norm_multi(*args) != 0
+    assert b"hrf_grad_norm_multi" in lib.hrf_last_error()
+
+
+def test_the_descriptor_has_the_header_s_layout():
+    from humanrf_amd import _lib
+    D = _lib.AdamWTensor
+    assert ctypes.sizeof(D) == 64
+    assert [getattr(D, f).offset for f in ("param", "grad", "copy", "n", "base", "first_tile", "kind", "lr_scale", "decay_scale")] == \
+        [0, 8, 16, 24, 32, 40, 44, 48, 56]
+
+
+def test_plans_refuse():
+    from humanrf_amd import ops
+    p = torch.zeros(8)
+    with pytest.raises(RuntimeError, match="no parameters"):
+        ops.AdamWPlan([])
+    with pytest.raises(RuntimeError, match="state_bits"):
+        ops.AdamWPlan([p], state_bits=4)
+    with pytest.raises(RuntimeError, match="negative"):
+        ops.AdamWPlan([p], step=-1)
+    with pytest.raises(RuntimeError, match="not on the expected device"):
+        ops.AdamWPlan([p])
+    with pytest.raises(RuntimeError, match="not contiguous"):
+        ops.AdamWPlan([torch.zeros(4, 4).t()])
+
+
+def test_the_optimizer_refuses():
+    from humanrf_amd.optim import AdamW
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="state_bits"):
+        AdamW([p], state_bits=16)
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        AdamW([p], max_grad_norm=0.0)
+    with pytest.raises(ValueError, match="betas and eps"):
+        AdamW([{"params": [p]}, {"params": [q], "eps": 1e-8}])
+    with pytest.raises(ValueError, match="tensor"):
+        AdamW([{"params": [p], "lr": torch.tensor(1.0)}, {"params": [q], "lr": torch.tensor(1.0)}])
+    opt = AdamW([p])
+    assert opt.step() is None           # no gradients: nothing to do, and nothing is built
+    p.grad = torch.zeros(4)
+    with pytest.raises(RuntimeError, match="not on the expected device"):
+        opt.step()
