@@ -18,6 +18,7 @@ _lock = threading.Lock()
 _lib = None
 
 HRF_MAX_LEVELS = 16
+ADAMW_CTL = 32 + 32 * 33   # HRF_ADAMW_CTL
 
 
 class LevelMeta(ctypes.Structure):
@@ -106,7 +107,7 @@ _SIGNATURES = {
     "hrf_adam_step": [_VP] * 5 + [_I64] + [_F] * 7 + [_VP, _VP],
     "hrf_adam_multi": [_VP, _I32, _I32, _I64] + [_F] * 5 + [_VP, _VP, _VP, _VP],
     "hrf_adamw_multi": [_VP, _VP, _I32, _I32, _I32] + [_VP] * 5 + [_D, _VP] + [_D] * 6 + [_VP] * 3 + [ctypes.c_uint32, _I32, _VP],
-    "hrf_grad_norm_multi": [_VP, _VP, _I32, _D] + [_VP] * 5,
+    "hrf_grad_norm_multi": [_VP, _VP, _I32, _D] + [_VP] * 4,
     "hrf_uniform_fill": [ctypes.c_uint32, _I64, _VP, _VP],
     "hrf_weights_fwd": [_VP] * 4 + [_I64, _VP, _VP],
     "hrf_weights_bwd": [_VP] * 5 + [_I64, _VP, _VP],

@@ -686,9 +686,9 @@ class AdamWPlan:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: build the plan before the capture of a graph")
         self.state = self._take_state(state)
-        self._ctl = torch.zeros(4 + len(params), dtype=torch.int32, device=self.device)
+        self._ctl = torch.zeros(_lib.ADAMW_CTL + len(params), dtype=torch.int32, device=self.device)
         if step:
-            self._ctl[4:] = int(step)
+            self._ctl[_lib.ADAMW_CTL:] = int(step)
         self._tile_tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), torch.tensor(tiles)).to(self.device)
         self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
         self._desc = None
@@ -745,12 +745,12 @@ class AdamWPlan:
     @property
     def steps(self) -> torch.Tensor:
         """int32 (tensors,), on the device: steps taken by each tensor."""
-        return self._ctl[4:]
+        return self._ctl[_lib.ADAMW_CTL:]
 
     @property
     def skipped(self) -> torch.Tensor:
         """int32 (1,), on the device: steps skipped for gradients that were not finite."""
-        return self._ctl[1:2]
+        return self._ctl[:1]
 
 
 def grad_norm_multi(plan: AdamWPlan, grad_scale: float = 1.0, scaler=None, out=None) -> torch.Tensor:
@@ -765,7 +765,7 @@ def grad_norm_multi(plan: AdamWPlan, grad_scale: float = 1.0, scaler=None, out=N
         raise RuntimeError("grad_norm_multi: the grad scaler lies on another device")
     with _on_device(plan.device), _span("grad_norm", plan.numel):
         check(_lib.lib().hrf_grad_norm_multi(ptr(plan._desc), ptr(plan._tile_tensor), plan.num_tiles, float(grad_scale), ptr(scaler),
-                                             ptr(plan._ctl), ptr(plan._ws), ptr(out), stream_ptr()))
+                                             ptr(plan._ws), ptr(out), stream_ptr()))
     return out
 
 

@@ -533,12 +533,14 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
  *   state_bits 32: exp_avg, second = fp32 moments m and v;
  *   state_bits 8:  exp_avg, second = e4m3 (OCP fn) codes of m and of sqrt(v), exp_avg_scale / second_scale = fp32, one per block. Codes
  *                  are rounded up or down at random, without bias, by a hash of (seed, step, position): the same call gives the same bits.
- * ctl: DEVICE int32[4 + count] = { internal, steps skipped, internal, internal, steps[count] }, zero at first. The launch advances the
- *   step counts of the tensors that have a gradient.
+ * ctl: DEVICE int32[HRF_ADAMW_CTL + count] = { steps skipped, internal ..., steps[count] }, zero at first. The launch advances the step
+ *   counts of the tensors that have a gradient.
  * lr: host value, or DEVICE fp32 lr_dev (may be NULL). Gradients are divided by grad_scale (times scaler->scale when a scaler is given)
  *   and, with max_norm > 0, multiplied by min(1, max_norm / (*norm + 1e-6)). The step is skipped (steps and values stay) when
  *   flags[0] != 0 or *norm (either may be NULL) is not finite; with a scaler its scale is then backed off, and grown as GradScaler does.
  * zero_grad != 0: the gradients are zeroed in the same pass. eps must be a positive normal fp32 number. */
+#define HRF_ADAMW_TICKETS 32
+#define HRF_ADAMW_CTL (32 + 32 * (1 + HRF_ADAMW_TICKETS)) /* counters of finished workgroups, each on a cache line of its own */
 typedef struct hrf_adamw_tensor {
     void* param;
     void* grad;        /* NULL: not stepped this time */
@@ -557,9 +559,9 @@ int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor,
                     double max_norm, const float* norm, const int32_t* flags, hrf_grad_scaler* scaler, uint32_t seed, int zero_grad,
                     hrf_stream_t stream);
 /* *out = 2-norm of all gradients of the tensors divided by grad_scale (times scaler->scale), summed in 64 bits in a fixed order.
- * workspace: DEVICE scratch of hrf_adamw_workspace_bytes() bytes; ctl as above. One norm or step of the same ctl at a time. */
+ * workspace: DEVICE scratch of hrf_adamw_workspace_bytes() bytes (one norm at a time). */
 int hrf_grad_norm_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor, int num_tiles, double grad_scale,
-                        const hrf_grad_scaler* scaler, int32_t* ctl, void* workspace, float* out, hrf_stream_t stream);
+                        const hrf_grad_scaler* scaler, void* workspace, float* out, hrf_stream_t stream);
 
 /* out[i] = value i of the counter-based uniform [0,1) stream `seed` (24 random bits, like torch.rand): the numbers
  * hrf_prune_march draws in-kernel for jitter_seed == seed. n < 2^32. */

@@ -37,10 +37,10 @@ def test_a_step_over_nothing_is_nothing():
 
 
 @pytest.mark.parametrize("args", [
-    (FAKE, FAKE, -1, 1.0, None, FAKE, FAKE, FAKE, None), (FAKE, FAKE, 1, 0.0, None, FAKE, FAKE, FAKE, None),
-    (FAKE, FAKE, 1, float("nan"), None, FAKE, FAKE, FAKE, None), (None, FAKE, 1, 1.0, None, FAKE, FAKE, FAKE, None),
-    (FAKE, None, 1, 1.0, None, FAKE, FAKE, FAKE, None), (FAKE, FAKE, 1, 1.0, None, None, FAKE, FAKE, None),
-    (FAKE, FAKE, 1, 1.0, None, FAKE, None, FAKE, None), (FAKE, FAKE, 1, 1.0, None, FAKE, FAKE, None, None),
+    (FAKE, FAKE, -1, 1.0, None, FAKE, FAKE, None), (FAKE, FAKE, 1, 0.0, None, FAKE, FAKE, None),
+    (FAKE, FAKE, 1, float("nan"), None, FAKE, FAKE, None), (None, FAKE, 1, 1.0, None, FAKE, FAKE, None),
+    (FAKE, None, 1, 1.0, None, FAKE, FAKE, None), (FAKE, FAKE, 1, 1.0, None, None, FAKE, None),
+    (FAKE, FAKE, 1, 1.0, None, FAKE, None, None),
 ])
 def test_the_norm_refuses(args):
     from humanrf_amd import _lib
