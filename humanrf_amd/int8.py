@@ -1,0 +1,75 @@
+"""Networks served with 8-bit weights over ops.linear_int8: layers of any width, next to the fused 64-neuron networks of the field model.
+Weights are rounded once (a scale for each channel), activations in every call (a scale for each row). For inference only."""
+from __future__ import annotations
+
+from typing import Sequence
+
+import torch
+
+from . import ops
+
+
+class Int8Linear(torch.nn.Module):
+    """y = act(x W^T + b), W in 8 bits: buffers `codes` (out, padded in), `scale` (out), `bias` (out) or None."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor = None, relu: bool = False):
+        super().__init__()
+        handle = ops.Int8Weight.from_float(weight, bias)
+        self.in_features, self.out_features, self.relu = handle.in_features, handle.out_features, bool(relu)
+        self.register_buffer("codes", handle.codes)
+        self.register_buffer("scale", handle.scale)
+        self.register_buffer("bias", handle.bias)
+        self._handle = handle
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, relu: bool = False) -> "Int8Linear":
+        return cls(linear.weight, linear.bias, relu)
+
+    def _apply(self, fn, recurse=True):
+        kept = (self.scale, self.bias)
+        out = super()._apply(fn, recurse)
+        # .half() / .bfloat16() cast floating buffers: scales and biases stay as they were, on the new device
+        for name, before in zip(("scale", "bias"), kept):
+            now = getattr(self, name)
+            if now is not None and now.dtype != torch.float32:
+                setattr(self, name, before.to(now.device))
+        self._handle = None
+        return out
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, out_dtype=None) -> torch.Tensor:
+        if self._handle is None:
+            self._handle = ops.Int8Weight.from_padded(self.codes, self.in_features, self.scale, self.bias)
+        return ops.linear_int8(x.detach(), self._handle, relu=self.relu, out_dtype=out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, relu={self.relu}"
+
+
+class Int8MLP(torch.nn.Sequential):
+    """Int8Linear layers one after the other, ReLU between them."""
+
+    @classmethod
+    def from_sequential(cls, net: torch.nn.Sequential) -> "Int8MLP":
+        """Linear layers, each followed by a ReLU or not."""
+        layers, mods = [], list(net)
+        for k, m in enumerate(mods):
+            if isinstance(m, torch.nn.Linear):
+                layers.append(Int8Linear.from_linear(m, relu=k + 1 < len(mods) and isinstance(mods[k + 1], torch.nn.ReLU)))
+            elif not (isinstance(m, torch.nn.ReLU) and k > 0 and isinstance(mods[k - 1], torch.nn.Linear)):
+                raise NotImplementedError(f"Int8MLP: only Linear layers, each with or without a ReLU behind it, got {type(m).__name__}")
+        return cls(*layers)
+
+    @classmethod
+    def from_flat(cls, params: torch.Tensor, widths: Sequence[int]) -> "Int8MLP":
+        """tcnn's flat parameter vector [w1 | ... | wL], row-major (widths[i + 1], widths[i]) matrices without biases, ReLU between them
+        (HumanRF.sigma_params: widths (32, 64, 16))."""
+        widths = [int(w) for w in widths]
+        sizes = [a * b for a, b in zip(widths[1:], widths[:-1])]
+        if len(widths) < 2 or min(widths) < 1 or params.numel() != sum(sizes):
+            raise RuntimeError(f"Int8MLP: widths {widths} take {sum(sizes)} parameters, got {params.numel()}")
+        parts = params.detach().reshape(-1).split(sizes)
+        return cls(*[Int8Linear(p.view(b, a), relu=k + 1 < len(sizes)) for k, (p, a, b) in enumerate(zip(parts, widths[:-1], widths[1:]))])
+
+
+__all__ = ["Int8Linear", "Int8MLP"]

@@ -800,6 +800,135 @@ def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weig
                                          1 if zero_grad else 0, stream_ptr()))
 
 
+_INT8_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+INT8_MAX_INNER = 131071
+
+
+def int8_padded(cols: int) -> int:
+    """Length that rows of `cols` 8-bit values are padded to with zeros: 64, or the next multiple of 128."""
+    return 64 if cols <= 64 else (cols + 127) // 128 * 128
+
+
+def _rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
+    """(rows, cols) view of (..., cols) values; rows may be further apart than they are long."""
+    if not t.is_cuda:
+        raise RuntimeError(f"Tensor is not on the expected device: {name}")
+    if t.dim() < 1 or not 1 <= t.shape[-1] <= INT8_MAX_INNER:
+        raise RuntimeError(f"{name}: 1 to {INT8_MAX_INNER} values a row, got shape {tuple(t.shape)}")
+    if t.dim() != 2:
+        if not t.is_contiguous():
+            raise RuntimeError(f"Tensor not contiguous: {name}")
+        t = t.view(-1, t.shape[-1])
+    if t.shape[0] > 0 and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        raise RuntimeError(f"Tensor not contiguous: {name} (within its rows)")
+    return t
+
+
+def quantize_int8(x: torch.Tensor):
+    """Rows of x (..., cols), float32 / float16 / bfloat16 -> (codes int8 (..., cols), scales float32 (...)): x ~ codes * scale, codes in
+    -127 .. 127 (hrf_quantize_rows_int8, include/hrf.h). The codes are a view of rows padded with zeros to int8_padded(cols). A row with
+    inf or NaN gets codes 0 and a scale that is not finite. Not differentiable."""
+    rows = _rows_of(x, "x")
+    if x.dtype not in _INT8_KINDS or x.dtype == torch.int8:
+        raise RuntimeError(f"quantize_int8: x must be float32, float16 or bfloat16, got {x.dtype}")
+    m, k = rows.shape
+    q = torch.empty(m, int8_padded(k), dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    with _on_device(x.device), _span("quantize_int8", m):
+        check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), _INT8_KINDS[x.dtype], m, k, rows.stride(0), ptr(q), q.shape[1], ptr(scale),
+                                                stream_ptr()))
+    return (q[:, :k] if x.dim() == 2 else q.view(*x.shape[:-1], q.shape[1])[..., :k]), scale.view(x.shape[:-1])
+
+
+def _padded_int8(rows: torch.Tensor) -> torch.Tensor:
+    """int8 rows as the product reads them: (rows, int8_padded(cols)), zeros behind the true length, 16-byte aligned; a copy unless
+    the rows lie like that already."""
+    m, k = rows.shape
+    if k == int8_padded(k) and rows.data_ptr() % 16 == 0 and (m == 1 or rows.stride(0) % 16 == 0):
+        return rows
+    q = torch.empty(m, int8_padded(k), dtype=torch.int8, device=rows.device)
+    with _on_device(rows.device):
+        check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), 3, m, k, rows.stride(0), ptr(q), q.shape[1], None, stream_ptr()))
+    return q
+
+
+class Int8Weight:
+    """A layer's weights for linear_int8, laid out once: codes int8 (channels, inner), one fp32 scale per channel, fp32 bias per channel
+    or None. Codes whose rows are whole multiples of the padded length are kept as they are (not copied); write new values through a new
+    handle. `from_float` rounds a weight matrix (channels, inner)."""
+
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        if codes.dim() != 2 or codes.dtype != torch.int8:
+            raise RuntimeError("Int8Weight: codes must be an int8 matrix (channels, inner)")
+        rows = _rows_of(codes, "codes")
+        self.out_features, self.in_features, self.device = codes.shape[0], codes.shape[1], codes.device
+        for t, name in ((scale, "scale"), (bias, "bias")):
+            if t is None:
+                continue
+            _chk(t, name, torch.float32)
+            if t.shape != (self.out_features,) or t.device != codes.device:
+                raise RuntimeError(f"Int8Weight: {name} must hold one value per channel on the codes' device")
+        self.codes, self.scale, self.bias = _padded_int8(rows), scale, bias
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Weight":
+        if weight.dim() != 2:
+            raise RuntimeError("Int8Weight: the weight must be a matrix (channels, inner)")
+        codes, scale = quantize_int8(weight.detach())
+        return cls(codes, scale, None if bias is None else bias.detach().float().contiguous())
+
+    @classmethod
+    def from_padded(cls, codes: torch.Tensor, in_features: int, scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Weight":
+        """`codes` (channels, int8_padded(in_features)) of another handle, zeros behind in_features: kept, not copied."""
+        if codes.dim() != 2 or codes.shape[1] != int8_padded(int(in_features)):
+            raise RuntimeError(f"Int8Weight: padded codes have {int8_padded(int(in_features))} values a row")
+        self = cls(codes, scale, bias)
+        self.in_features = int(in_features)
+        return self
+
+
+def linear_int8(x: torch.Tensor, weight: Int8Weight, x_scale: Optional[torch.Tensor] = None, relu: bool = False, out_dtype=None) -> torch.Tensor:
+    """act(x W^T + bias) with W in 8-bit integers (hrf_linear_int8, include/hrf.h) -> (..., channels). x (..., inner): float32, float16 or
+    bfloat16, rounded to 8 bits with a scale of its own for each row; or int8 codes with x_scale (...) fp32. Rows may be further apart
+    than they are long. out_dtype: float32, float16 or bfloat16 (default: x's own, float32 for codes). Serving only: no gradients flow."""
+    rows = _rows_of(x, "x")
+    m, k = rows.shape
+    if k != weight.in_features:
+        raise RuntimeError(f"linear_int8: x has {k} values a row, the weight {weight.in_features}")
+    if x.device != weight.device:
+        raise RuntimeError("linear_int8: x and the weight lie on different devices")
+    if x.dtype not in _INT8_KINDS:
+        raise RuntimeError(f"linear_int8: x must be float32, float16, bfloat16 or int8, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("linear_int8: no gradient flows through the product; call it under torch.no_grad()")
+    if (x.dtype == torch.int8) != (x_scale is not None):
+        raise RuntimeError("linear_int8: x_scale comes with int8 codes, and only with them")
+    if out_dtype is None:
+        out_dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
+    if out_dtype not in _ADAMW_KINDS:
+        raise RuntimeError(f"linear_int8: out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    if x_scale is not None:
+        _chk(x_scale, "x_scale", torch.float32)
+        if x_scale.numel() != m or x_scale.device != x.device:
+            raise RuntimeError("linear_int8: one x_scale for each row, on x's device")
+    y = torch.empty(*x.shape[:-1], weight.out_features, dtype=out_dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    with _on_device(x.device), _span("linear_int8", m):
+        if x_scale is None:
+            codes = torch.empty(m, int8_padded(k), dtype=torch.int8, device=x.device)
+            x_scale = torch.empty(m, dtype=torch.float32, device=x.device)
+            check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), _INT8_KINDS[x.dtype], m, k, rows.stride(0), ptr(codes), codes.shape[1],
+                                                    ptr(x_scale), stream_ptr()))
+        else:
+            codes = _padded_int8(rows)
+        w = weight.codes
+        check(_lib.lib().hrf_linear_int8(ptr(codes), codes.stride(0), ptr(x_scale), ptr(w), w.stride(0), ptr(weight.scale), ptr(weight.bias),
+                                         m, weight.out_features, w.shape[1], ptr(y), _INT8_KINDS[out_dtype], weight.out_features,
+                                         1 if relu else 0, stream_ptr()))
+    return y
+
+
 def compose_forward(xyz_f, xyt_f, yzt_f, xzt_f, vectors, xyzt):
     for a, nm in ((xyz_f, "xyz_features"), (xyt_f, "xyt_features"), (yzt_f, "yzt_features"), (xzt_f, "xzt_features")):
         _chk(a, nm, torch.float16)

@@ -563,6 +563,23 @@ int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor,
 int hrf_grad_norm_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_tensor, int num_tiles, double grad_scale,
                         const hrf_grad_scaler* scaler, void* workspace, float* out, hrf_stream_t stream);
 
+/* ------------------------------------------------------------------ 8-bit integer product -- */
+/* y[m][n] = act((sum_k x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]): a layer served with 8-bit weights, a scale for each
+ * channel n and each token m; integer sums are exact. No counterpart in the reference, whose networks are fp16 (humanrf.py:123-156).
+ * x (rows, inner), w (cols, inner) int8, row strides ldx, ldw: both begin at multiples of 16 bytes, `inner` is a padded length
+ * (hrf_int8_padded: 64, or a multiple of 128; HRF_INT8_MAX_INNER before padding keeps the sums inside int32) and the bytes from the true length to `inner`
+ * are zero. bias (cols) fp32 or NULL; relu != 0: max(., 0). y: row stride ldy (in values), y_type 0 fp32, 1 fp16, 2 bf16. */
+#define HRF_INT8_MAX_INNER 131071
+int64_t hrf_int8_padded(int64_t cols);
+int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                    const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
+                    hrf_stream_t stream);
+/* Rows of x (x_type 0 fp32, 1 fp16, 2 bf16; row stride ldx) -> codes q (row stride ldq >= cols, filled with zeros behind cols) and one
+ * scale a row: scale = a * (1 / 127), q = rint(x * (127 / a)), a = max(max |x|, 2^-119). A row that is not finite gets codes 0 and a
+ * scale that is not finite. x_type 3: int8 rows are copied, with the padding (scale is not written and may be NULL). */
+int hrf_quantize_rows_int8(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                           hrf_stream_t stream);
+
 /* out[i] = value i of the counter-based uniform [0,1) stream `seed` (24 random bits, like torch.rand): the numbers
  * hrf_prune_march draws in-kernel for jitter_seed == seed. n < 2^32. */
 int hrf_uniform_fill(uint32_t seed, int64_t n, float* out, hrf_stream_t stream);

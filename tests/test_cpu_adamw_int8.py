@@ -88,3 +88,68 @@ def test_the_optimizer_refuses():
     p.grad = torch.zeros(4)
     with pytest.raises(RuntimeError, match="not on the expected device"):
         opt.step()
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit integer product
+def _linear(lib, **change):
+    a = dict(x=FAKE, ldx=128, x_scale=FAKE, w=FAKE, ldw=128, w_scale=FAKE, bias=None, rows=4, cols=8, inner=128, y=FAKE, y_type=0, ldy=8,
+             relu=0, stream=None)
+    a.update(change)
+    return lib.hrf_linear_int8(*a.values())
+
+
+@pytest.mark.parametrize("change,said", [
+    (dict(y_type=3), b"y_type"), (dict(y_type=-1), b"y_type"), (dict(rows=-1), b"sizes"), (dict(cols=-1), b"sizes"),
+    (dict(rows=2 ** 31), b"sizes"), (dict(inner=0), b"inner"), (dict(inner=100), b"inner"), (dict(inner=192), b"inner"),
+    (dict(inner=131200, ldx=131200, ldw=131200), b"inner"), (dict(x=None), b"NULL"), (dict(w=None), b"NULL"), (dict(y=None), b"NULL"),
+    (dict(x_scale=None), b"NULL"), (dict(w_scale=None), b"NULL"), (dict(ldx=64), b"stride"), (dict(ldw=112), b"stride"),
+    (dict(ldy=7), b"stride"), (dict(ldx=136), b"multiples of 16"), (dict(x=FAKE + 8), b"multiples of 16"), (dict(w=FAKE + 1), b"multiples of 16"),
+])
+def test_the_product_refuses(change, said):
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    assert _linear(lib, **change) != 0
+    assert b"hrf_linear_int8" in lib.hrf_last_error() and said in lib.hrf_last_error()
+
+
+def test_products_of_nothing_are_nothing():
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    assert _linear(lib, rows=0, x=None, y=None) == 0 and _linear(lib, cols=0, w=None, y=None) == 0
+    assert lib.hrf_quantize_rows_int8(None, 0, 0, 5, 5, None, 64, None, None) == 0
+
+
+@pytest.mark.parametrize("args", [
+    (FAKE, 4, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, -1, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, 0, -1, 5, 5, FAKE, 64, FAKE, None),
+    (FAKE, 0, 2, 0, 5, FAKE, 64, FAKE, None), (FAKE, 0, 2, 131072, 131072, FAKE, 131072, FAKE, None), (None, 0, 2, 5, 5, FAKE, 64, FAKE, None),
+    (FAKE, 0, 2, 5, 5, None, 64, FAKE, None), (FAKE, 0, 2, 5, 5, FAKE, 64, None, None), (FAKE, 0, 2, 5, 4, FAKE, 64, FAKE, None),
+    (FAKE, 0, 2, 5, 5, FAKE, 4, FAKE, None),
+])
+def test_rounding_rows_refuses(args):
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    assert lib.hrf_quantize_rows_int8(*args) != 0
+    assert b"hrf_quantize_rows_int8" in lib.hrf_last_error()
+
+
+def test_padded_lengths():
+    from humanrf_amd import _lib, ops
+    lib = _lib.lib()
+    assert [lib.hrf_int8_padded(k) for k in (0, 131072)] == [-1, -1]
+    for k in (1, 63, 64, 65, 127, 128, 129, 2051, 131071):
+        assert lib.hrf_int8_padded(k) == ops.int8_padded(k) >= k
+
+
+def test_the_wrappers_refuse():
+    from humanrf_amd import int8, ops
+    x = torch.zeros(3, 8)
+    with pytest.raises(RuntimeError, match="not on the expected device"):
+        ops.quantize_int8(x)
+    with pytest.raises(RuntimeError, match="int8 matrix"):
+        ops.Int8Weight(x, torch.ones(3))
+    with pytest.raises(RuntimeError, match="must be a matrix"):
+        ops.Int8Weight.from_float(x[0])
+    with pytest.raises(NotImplementedError, match="Sigmoid"):
+        int8.Int8MLP.from_sequential(torch.nn.Sequential(torch.nn.Sigmoid()))
+    with pytest.raises(RuntimeError, match="parameters"):
+        int8.Int8MLP.from_flat(x, (4, 4))
