@@ -844,7 +844,7 @@ def _padded_int8(rows: torch.Tensor) -> torch.Tensor:
     """int8 rows as the product reads them: (rows, int8_padded(cols)), zeros behind the true length, 16-byte aligned; a copy unless
     the rows lie like that already."""
     m, k = rows.shape
-    if k == int8_padded(k) and rows.data_ptr() % 16 == 0 and (m == 1 or rows.stride(0) % 16 == 0):
+    if k == int8_padded(k) and rows.data_ptr() % 16 == 0 and (m == 1 or (rows.stride(0) % 16 == 0 and rows.stride(0) < 1 << 23)):
         return rows
     q = torch.empty(m, int8_padded(k), dtype=torch.int8, device=rows.device)
     with _on_device(rows.device):

@@ -570,6 +570,7 @@ int hrf_grad_norm_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_ten
  * (hrf_int8_padded: 64, or a multiple of 128; HRF_INT8_MAX_INNER before padding keeps the sums inside int32) and the bytes from the true length to `inner`
  * are zero. bias (cols) fp32 or NULL; relu != 0: max(., 0). y: row stride ldy (in values), y_type 0 fp32, 1 fp16, 2 bf16. */
 #define HRF_INT8_MAX_INNER 131071
+#define HRF_INT8_MAX_STRIDE (1 << 23) /* row strides of x and w are smaller; cols is at most 64 * 65535 */
 int64_t hrf_int8_padded(int64_t cols);
 int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                     const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
