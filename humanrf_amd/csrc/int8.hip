@@ -23,27 +23,99 @@ template <> struct I8Type<I8_F16> { typedef __half T; static __device__ float up
 template <> struct I8Type<I8_BF16> { typedef __bf16 T; static __device__ float up(__bf16 x) { return (float)x; } static __device__ __bf16 down(float x) { return (__bf16)x; } };
 
 // ------------------------------------------------------------------------------------------------ rows -> codes and scales
-// One workgroup a row. A row that is not finite gets a scale that is not, and codes 0: its outputs are NaN.
-template <int K>
-__global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>::T* __restrict__ x, int64_t cols, int64_t ldx,
+// One 16-byte piece of a row, as fp32.
+template <int K> struct alignas(16) I8Piece { static constexpr int n = 16 / (int)sizeof(typename I8Type<K>::T); typename I8Type<K>::T v[16 / sizeof(typename I8Type<K>::T)]; };
+
+__device__ __forceinline__ uint32_t i8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }     // |x| as an integer: the order of the values, NaN on top
+
+// amax -> factor of the codes and stored scale. A row that is not finite gets a scale that is not, and codes 0: its outputs are NaN.
+__device__ __forceinline__ float i8_factor(uint32_t top, float& scale)
+{
+    const float amax = __uint_as_float(max(top, 0x04000000u));      // 2^-119: 127 / amax stays finite, a row of zeros gives zeros
+    scale = amax * (1.0f / 127.0f);
+    return top < 0x7f800000u ? 127.0f / amax : 0.0f;
+}
+
+// Four values -> four codes in one word. |x| * factor is below 127.0001 (and 0 * NaN converts to 0), so that no clamp is needed.
+__device__ __forceinline__ uint32_t i8_code(float x, float factor, bool finite) { return finite ? (uint32_t)(int)rintf(x * factor) & 0xffu : 0u; }
+
+// kGroup lanes (a power of two, or the whole workgroup of 256 in groups of 64 joined through LDS) a row; the row is read once and stays in
+// registers, kPieces 16-byte pieces a lane. Both sides of that: rows of 4096 bf16 from memory twice, value by value, 118 us for 8192
+// of them; this way 35 us.
+template <int K, int kGroup, int kPieces>
+__global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>::T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                        int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
+{
+    __shared__ uint32_t s_max[4];
+    constexpr int n = I8Piece<K>::n, kRows = 256 / kGroup;
+    const int lane = threadIdx.x % kGroup;
+    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kGroup;
+    const bool here = row < rows;
+    const typename I8Type<K>::T* const from = x + (here ? row : rows - 1) * ldx;
+    I8Piece<K> v[kPieces];
+    uint32_t top = 0;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        const int k0 = (p * kGroup + lane) * n;
+        if (k0 + n <= cols) v[p] = *(const I8Piece<K>*)(from + k0);
+        else {
+#pragma unroll
+            for (int k = 0; k < n; ++k) v[p].v[k] = k0 + k < cols ? from[k0 + k] : I8Type<K>::down(0.0f);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int k = 0; k < n; ++k) top = max(top, i8_bits(I8Type<K>::up(v[p].v[k])));
+#pragma unroll
+    for (int s = (kGroup < 64 ? kGroup : 64) / 2; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    if (kGroup == 256) {
+        if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    }
+    if (!here) return;
+    float sc;
+    const float factor = i8_factor(top, sc);
+    const bool finite = top < 0x7f800000u;
+    if (lane == 0) scale[row] = sc;
+    int8_t* const to = q + row * ldq;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        const int k0 = (p * kGroup + lane) * n;
+        if (k0 >= ldq) continue;        // (the padding up to ldq is a multiple of 64 away: whole pieces)
+        uint32_t word[n / 4];
+#pragma unroll
+        for (int w = 0; w < n / 4; ++w) {
+            word[w] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) word[w] |= i8_code(I8Type<K>::up(v[p].v[4 * w + k]), factor, finite) << (8 * k);
+        }
+        if (n == 8) *(uint2*)(to + k0) = make_uint2(word[0], word[n / 4 - 1]);
+        else *(uint32_t*)(to + k0) = word[0];
+    }
+}
+
+// Rows at addresses that are no multiples of 16 bytes, or longer than 16384: value by value, twice.
+template <int K>
+__global__ __launch_bounds__(256) void k_quantize_rows_any(const typename I8Type<K>::T* __restrict__ x, int64_t cols, int64_t ldx,
+                                                           int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
 {
     __shared__ uint32_t s_max[4];
     x += (int64_t)blockIdx.x * ldx;
     q += (int64_t)blockIdx.x * ldq;
-    uint32_t top = 0;       // of |x| as integers: the order of the values, NaN on top
-    for (int64_t k = threadIdx.x; k < cols; k += 256) top = max(top, __float_as_uint(I8Type<K>::up(x[k])) & 0x7fffffffu);
+    uint32_t top = 0;
+    for (int64_t k = threadIdx.x; k < cols; k += 256) top = max(top, i8_bits(I8Type<K>::up(x[k])));
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
     __syncthreads();
     top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    float sc;
+    const float factor = i8_factor(top, sc);
     const bool finite = top < 0x7f800000u;
-    const float amax = __uint_as_float(max(top, 0x04000000u));      // 2^-119: 127 / amax stays finite, a row of zeros gives zeros
-    const float inverse = finite ? 127.0f / amax : 0.0f;
-    if (threadIdx.x == 0) scale[blockIdx.x] = amax * (1.0f / 127.0f);
-    for (int64_t k = threadIdx.x; k < ldq; k += 256)
-        q[k] = k < cols && finite ? (int8_t)(int)rintf(I8Type<K>::up(x[k]) * inverse) : (int8_t)0;
+    if (threadIdx.x == 0) scale[blockIdx.x] = sc;
+    for (int64_t k = threadIdx.x; k < ldq; k += 256) q[k] = k < cols ? (int8_t)i8_code(I8Type<K>::up(x[k]), factor, finite) : (int8_t)0;
 }
 
 __global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, int64_t cols, int64_t ldx, int8_t* __restrict__ q, int64_t ldq)
@@ -230,50 +302,187 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
     }
 }
 
-// Rows of 64 bytes (inner <= 64): one instruction's k. A wavefront keeps the fragments of 64 channels in registers and walks over blocks of
-// 16 tokens, whose operands come straight from memory.
-template <int K>
-__global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A)
+// Short rows (up to 64 KS values), many of them: bound by the bytes of x and y, so x is rounded on its way in and nothing is written
+// between. A wavefront keeps the weights of 64 channels in registers and walks over blocks of 16 tokens; lane (t, q) = (lane & 15, lane >> 4)
+// holds 16 values of token t for each 64, finds the row's largest with the three other lanes of the token, and has its operand. The
+// channels are dealt to the instructions so that a lane's 16 results are 16 neighbouring channels of one token: 32 bytes of fp16 in a
+// row of 128.
+struct I8Short {
+    const void* x;
+    int64_t ldx;
+    int inner;              // not padded
+    int x_wide, y_wide;     // rows of x / y begin at multiples of 16 bytes
+};
+
+template <int X, int K, int KS>
+__global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A, const I8Short B)
 {
     typedef typename I8Type<K>::T T;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
     const int waves = (int)gridDim.x * 4, wave = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
     const int n0 = (int)blockIdx.y * 64;
     const bool has_bias = A.bias != nullptr, relu = A.relu != 0;
-    i8_v4 fw[4];
-    float sw[4][4], bias[4][4];
+    i8_v4 fw[KS][4];
+    float sw[16], bias[16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-        const int row = min(n0 + a * 16 + (lane & 15), A.cols - 1);
-        fw[a] = *(const i8_v4*)(A.w + (int64_t)row * A.ldw + (lane >> 4) * 16);
+        const int row = min(n0 + (t >> 2) * 16 + a * 4 + (t & 3), A.cols - 1);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int n = min(n0 + a * 16 + (lane >> 4) * 4 + k, A.cols - 1);
-            sw[a][k] = A.sw[n];
-            bias[a][k] = has_bias ? A.bias[n] : 0.0f;
-        }
+        for (int s = 0; s < KS; ++s) fw[s][a] = *(const i8_v4*)(A.w + (int64_t)row * A.ldw + s * 64 + q * 16);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int n = min(n0 + q * 16 + k, A.cols - 1);
+        sw[k] = A.sw[n];
+        bias[k] = has_bias ? A.bias[n] : 0.0f;
     }
     const int blocks = (A.rows + 15) / 16;
     for (int blk = wave; blk < blocks; blk += waves) {
-        const int m = blk * 16 + (lane & 15), row = min(m, A.rows - 1);
-        const i8_v4 fx = *(const i8_v4*)(A.x + (int64_t)row * A.ldx + (lane >> 4) * 16);
-        const float sx = A.sx[row];
-        T* const y = (T*)A.y + (int64_t)row * A.ldy;
+        const int m = blk * 16 + t;
+        const int64_t row = min(m, A.rows - 1);
+        i8_v4 fx[KS];
+        float sx;
+        if constexpr (X == I8_INT8) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) fx[s] = *(const i8_v4*)((const int8_t*)B.x + row * B.ldx + s * 64 + q * 16);
+            sx = A.sx[row];
+        } else {
+            typedef typename I8Type<X>::T XT;
+            constexpr int n = I8Piece<X>::n, kPieces = 16 / n;
+            const XT* const from = (const XT*)B.x + row * B.ldx;
+            I8Piece<X> v[KS][kPieces];
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int p = 0; p < kPieces; ++p) {
+                    const int k0 = s * 64 + q * 16 + p * n;
+                    if (B.x_wide && k0 + n <= B.inner) v[s][p] = *(const I8Piece<X>*)(from + k0);
+                    else {
+#pragma unroll
+                        for (int k = 0; k < n; ++k) v[s][p].v[k] = k0 + k < B.inner ? from[k0 + k] : I8Type<X>::down(0.0f);
+                    }
+                }
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+                    for (int k = 0; k < n; ++k) top = max(top, i8_bits(I8Type<X>::up(v[s][p].v[k])));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+            const float factor = i8_factor(top, sx);
+            const bool finite = top < 0x7f800000u;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t word = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) word |= i8_code(I8Type<X>::up(v[s][(4 * w + k) / n].v[(4 * w + k) % n]), factor, finite) << (8 * k);
+                    fx[s][w] = (int)word;
+                }
+        }
+        __align__(16) T out[16];
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const i8_v4 acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[a], fx, i8_v4{0, 0, 0, 0}, 0, 0, 0);
-            const int n = n0 + a * 16 + (lane >> 4) * 4;
+            i8_v4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (m < A.rows && n + k < A.cols) y[n + k] = i8_finish<K>(acc[k], sx, sw[a][k], bias[a][k], has_bias, relu);
+            for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[s][a], fx[s], acc, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out[a * 4 + k] = i8_finish<K>(acc[k], sx, sw[a * 4 + k], bias[a * 4 + k], has_bias, relu);
+        }
+        if (m >= A.rows) continue;
+        const int n = n0 + q * 16;
+        T* const y = (T*)A.y + row * A.ldy + n;
+        if (B.y_wide && n + 16 <= A.cols) {
+#pragma unroll
+            for (int p = 0; p < (int)sizeof(T); ++p) ((i8_v4*)y)[p] = ((const i8_v4*)out)[p];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (n + k < A.cols) y[k] = out[k];
         }
     }
 }
 
-template <int K>
-static void i8_quantize(const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, hipStream_t stream)
+// Few tokens (up to 16 MT): bound by the bytes of W, which every workgroup reads its part of once: 16 NT channels, the k axis dealt to its
+// kWaves wavefronts in runs of 64 bytes, sums joined in LDS. Integer sums: any order gives the same.
+template <int K, int MT, int NT, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void k_linear_i8_few(const I8Args A)
 {
-    hipLaunchKernelGGL(k_quantize_rows<K>, dim3((unsigned)rows), dim3(256), 0, stream, (const typename I8Type<K>::T*)x, cols, ldx, q, ldq, scale);
+    typedef typename I8Type<K>::T T;
+    __shared__ i8_v4 s_part[kWaves][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = lane & 15, q = lane >> 4;
+    const int n0 = (int)blockIdx.x * 16 * NT;
+    const int runs = A.inner >> 6, each = (runs + kWaves - 1) / kWaves, begin = wave * each, end = min(begin + each, runs);
+    const int8_t* w[NT];
+    const int8_t* x[MT];
+#pragma unroll
+    for (int a = 0; a < NT; ++a) w[a] = A.w + (int64_t)min(n0 + a * 16 + t, A.cols - 1) * A.ldw + q * 16;
+#pragma unroll
+    for (int b = 0; b < MT; ++b) x[b] = A.x + (int64_t)min(b * 16 + t, A.rows - 1) * A.ldx + q * 16;
+    i8_v4 acc[NT][MT];
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int b = 0; b < MT; ++b) acc[a][b] = i8_v4{0, 0, 0, 0};
+    constexpr int kAhead = MT * NT > 4 ? 2 : MT * NT > 1 ? 4 : 8;        // runs on their way at a time
+    for (int r = begin; r < end; r += kAhead) {
+        i8_v4 fw[kAhead][NT], fx[kAhead][MT];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t k = (int64_t)min(r + u, end - 1) * 64;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) fw[u][a] = __builtin_nontemporal_load((const i8_v4*)(w[a] + k));
+#pragma unroll
+            for (int b = 0; b < MT; ++b) fx[u][b] = *(const i8_v4*)(x[b] + k);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (r + u < end) {
+#pragma unroll
+                for (int a = 0; a < NT; ++a)
+#pragma unroll
+                    for (int b = 0; b < MT; ++b) acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u][a], fx[u][b], acc[a][b], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int b = 0; b < MT; ++b) s_part[wave][a * MT + b][lane] = acc[a][b];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 256 * MT * NT; e += 64 * kWaves) {
+        const int n = n0 + e % (16 * NT), m = e / (16 * NT);       // neighbouring threads: neighbouring channels of one token
+        if (m >= A.rows || n >= A.cols) continue;
+        const int nl = (n - n0) & 15, tile = ((n - n0) >> 4) * MT + (m >> 4), from = (nl >> 2) * 16 + (m & 15);
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) sum += s_part[v][tile][from][nl & 3];
+        ((T*)A.y)[(int64_t)m * A.ldy + n] = i8_finish<K>(sum, A.sx[m], A.sw[n], A.bias ? A.bias[n] : 0.0f, A.bias != nullptr, A.relu != 0);
+    }
+}
+
+template <int K>
+static void i8_quantize(const void* xv, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, hipStream_t stream)
+{
+    typedef typename I8Type<K>::T T;
+    const T* x = (const T*)xv;
+    constexpr int n = I8Piece<K>::n;
+    const int64_t width = std::max(cols, ldq);
+    // whole pieces: rows of x at multiples of 16 bytes, rows of q at multiples of 8 and padded to them
+    const bool pieces = (((uintptr_t)x | (uintptr_t)(ldx * (int64_t)sizeof(T))) & 15u) == 0 && (((uintptr_t)q | (uintptr_t)ldq) & 7u) == 0;
+#define I8_ROWS(G, P)                                                                                                            \
+    hipLaunchKernelGGL((k_quantize_rows<K, G, P>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))), dim3(256), 0, stream, x, rows, \
+                       (int)cols, ldx, q, ldq, scale)
+    if (!pieces || width > 256 * 8 * n)
+        hipLaunchKernelGGL(k_quantize_rows_any<K>, dim3((unsigned)rows), dim3(256), 0, stream, x, cols, ldx, q, ldq, scale);
+    else if (width <= 16 * n) I8_ROWS(16, 1);
+    else if (width <= 64 * n) I8_ROWS(64, 1);
+    else if (width <= 64 * 4 * n) I8_ROWS(64, 4);
+    else if (width <= 256 * 4 * n) I8_ROWS(256, 4);
+    else I8_ROWS(256, 8);
+#undef I8_ROWS
 }
 
 static int i8_padded(int64_t cols) { return (int)(cols <= 64 ? 64 : (cols + 127) / 128 * 128); }
@@ -296,15 +505,37 @@ extern "C" int hrf_quantize_rows_int8(const void* x, int x_type, int64_t rows, i
     return 0;
 }
 
+static bool i8_wide(const void* p, int64_t ld, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & 15u) == 0; }
+
+// Rows of up to 256 values and up to 128 channels, when there are enough rows to fill the card.
+static bool i8_is_short(int64_t rows, int64_t cols, int64_t inner) { return inner == 64 || (inner <= 256 && cols <= 128 && rows > 4096); }
+
+template <int X, int K>
+static void i8_short(const I8Args& A, const void* x, int64_t ldx, int64_t inner, int size, hipStream_t stream)
+{
+    I8Short B;
+    B.x = x; B.ldx = ldx; B.inner = (int)inner; B.x_wide = i8_wide(x, ldx, size); B.y_wide = i8_wide(A.y, A.ldy, (int)sizeof(typename I8Type<K>::T));
+    const dim3 grid((unsigned)std::min<int64_t>((A.rows + 63) / 64, 2048), (unsigned)((A.cols + 63) / 64));
+    if (A.inner == 64) hipLaunchKernelGGL((k_linear_i8_short<X, K, 1>), grid, dim3(256), 0, stream, A, B);
+    else if (A.inner == 128) hipLaunchKernelGGL((k_linear_i8_short<X, K, 2>), grid, dim3(256), 0, stream, A, B);
+    else hipLaunchKernelGGL((k_linear_i8_short<X, K, 4>), grid, dim3(256), 0, stream, A, B);
+}
+
+template <int K, int MT, int NT>
+static void i8_few(const I8Args& A, hipStream_t stream)
+{
+    const dim3 grid((unsigned)((A.cols + 16 * NT - 1) / (16 * NT)));
+    if (A.inner >= 2048) hipLaunchKernelGGL((k_linear_i8_few<K, MT, NT, 8>), grid, dim3(512), 0, stream, A);
+    else hipLaunchKernelGGL((k_linear_i8_few<K, MT, NT, 4>), grid, dim3(256), 0, stream, A);
+}
+
 template <int K>
 static void i8_linear(const I8Args& A, hipStream_t stream)
 {
-    if (A.inner == 64) {
-        const int64_t waves = ((int64_t)A.rows + 15) / 16;
-        const unsigned blocks = (unsigned)std::min<int64_t>((waves + 3) / 4, 2048);
-        hipLaunchKernelGGL((k_linear_i8_short<K>), dim3(blocks, (unsigned)((A.cols + 63) / 64)), dim3(256), 0, stream, A);
-        return;
-    }
+    if (i8_is_short(A.rows, A.cols, A.inner)) { i8_short<I8_INT8, K>(A, A.x, A.ldx, A.inner, 1, stream); return; }
+    if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
+    if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
+    if (A.rows <= 64) { i8_few<K, 4, 2>(A, stream); return; }
     const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256);
     if (large >= 200) hipLaunchKernelGGL((k_linear_i8<K, 4, 4>), dim3((unsigned)large), dim3(256), 0, stream, A);
     else {
@@ -313,25 +544,82 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     }
 }
 
+#define I8_CHECK(cond, msg)                      \
+    do {                                         \
+        if (!(cond)) {                           \
+            hrf_set_error("%s: %s", name, msg);  \
+            return 1;                            \
+        }                                        \
+    } while (0)
+static int i8_check(const char* name, const void* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
+                    int64_t rows, int64_t cols, int64_t inner, const void* y, int y_type, int64_t ldy)
+{
+    I8_CHECK(y_type >= I8_F32 && y_type <= I8_BF16, "y_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    I8_CHECK(rows >= 0 && rows < ((int64_t)1 << 31) - 256 && cols >= 0 && cols < ((int64_t)1 << 31) - 256, "bad sizes");
+    I8_CHECK(inner >= 64 && inner <= HRF_INT8_MAX_INNER + 1 && inner == i8_padded(inner), "inner must be a padded length (hrf_int8_padded)");
+    if (rows == 0 || cols == 0) return 0;
+    I8_CHECK(x && x_scale && w && w_scale && y, "NULL argument");
+    I8_CHECK((ldx >= inner || rows == 1) && (ldw >= inner || cols == 1) && (ldy >= cols || rows == 1), "a row stride is shorter than the row");
+    I8_CHECK((((uintptr_t)x | (uintptr_t)w) & 15u) == 0 && ((ldx | ldw) & 15) == 0, "x and w and their rows must begin at multiples of 16 bytes");
+    I8_CHECK(ldx < HRF_INT8_MAX_STRIDE && ldw < HRF_INT8_MAX_STRIDE, "rows are too far apart");
+    I8_CHECK(((rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 31) && cols <= 64 * 65535, "too many tiles");
+    return 0;
+}
+
 extern "C" int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                                const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
                                hrf_stream_t stream)
 {
-    HRF_CHECK_ARG(y_type >= I8_F32 && y_type <= I8_BF16, "y_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
-    HRF_CHECK_ARG(rows >= 0 && rows < ((int64_t)1 << 31) - 256 && cols >= 0 && cols < ((int64_t)1 << 31) - 256, "bad sizes");
-    HRF_CHECK_ARG(inner >= 64 && inner <= HRF_INT8_MAX_INNER + 1 && inner == i8_padded(inner), "inner must be a padded length (hrf_int8_padded)");
-    if (rows == 0 || cols == 0) return 0;
-    HRF_CHECK_ARG(x && x_scale && w && w_scale && y, "NULL argument");
-    HRF_CHECK_ARG((ldx >= inner || rows == 1) && (ldw >= inner || cols == 1) && (ldy >= cols || rows == 1), "a row stride is shorter than the row");
-    HRF_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15u) == 0 && ((ldx | ldw) & 15) == 0, "x and w and their rows must begin at multiples of 16 bytes");
-    HRF_CHECK_ARG(ldx < HRF_INT8_MAX_STRIDE && ldw < HRF_INT8_MAX_STRIDE, "rows are too far apart");
-    HRF_CHECK_ARG(((rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 31) && cols <= 64 * 65535, "too many tiles");
+    const int rc = i8_check(__func__, x, ldx, x_scale, w, ldw, w_scale, rows, cols, inner, y, y_type, ldy);
+    if (rc || rows == 0 || cols == 0) return rc;
     I8Args A;
     A.x = x; A.w = w; A.sx = x_scale; A.sw = w_scale; A.bias = bias; A.y = y; A.ldx = ldx; A.ldw = ldw; A.ldy = ldy;
     A.rows = (int)rows; A.cols = (int)cols; A.inner = (int)inner; A.relu = relu;
     if (y_type == I8_F32) i8_linear<I8_F32>(A, (hipStream_t)stream);
     else if (y_type == I8_F16) i8_linear<I8_F16>(A, (hipStream_t)stream);
     else i8_linear<I8_BF16>(A, (hipStream_t)stream);
+    HRF_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int X>
+static void i8_float(const I8Args& A, const void* x, int64_t ldx, int64_t inner, int y_type, hipStream_t stream)
+{
+    constexpr int size = (int)sizeof(typename I8Type<X>::T);
+    if (y_type == I8_F32) i8_short<X, I8_F32>(A, x, ldx, inner, size, stream);
+    else if (y_type == I8_F16) i8_short<X, I8_F16>(A, x, ldx, inner, size, stream);
+    else i8_short<X, I8_BF16>(A, x, ldx, inner, size, stream);
+}
+
+extern "C" int64_t hrf_linear_int8_workspace_bytes(int64_t rows, int64_t cols, int64_t inner)
+{
+    if (rows <= 0 || cols <= 0 || inner < 1 || inner > HRF_INT8_MAX_INNER) return 0;
+    return i8_is_short(rows, cols, i8_padded(inner)) ? 0 : rows * i8_padded(inner) + ((rows * 4 + 15) & ~(int64_t)15);
+}
+
+extern "C" int hrf_linear_int8_float(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                                     int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu, void* workspace,
+                                     hrf_stream_t stream)
+{
+    HRF_CHECK_ARG(x_type >= I8_F32 && x_type <= I8_BF16, "x_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    HRF_CHECK_ARG(inner >= 1 && inner <= HRF_INT8_MAX_INNER, "bad sizes");
+    const int64_t need = hrf_linear_int8_workspace_bytes(rows, cols, inner), padded = i8_padded(inner);
+    int rc = i8_check(__func__, (const void*)16, padded, (const float*)16, w, ldw, w_scale, rows, cols, padded, y, y_type, ldy);
+    if (rc || rows == 0 || cols == 0) return rc;
+    HRF_CHECK_ARG(x, "NULL argument");
+    HRF_CHECK_ARG(ldx >= inner || rows == 1, "a row stride is shorter than the row");
+    if (need > 0) {
+        HRF_CHECK_ARG(workspace && ((uintptr_t)workspace & 15u) == 0, "the workspace must begin at a multiple of 16 bytes");
+        float* const scale = (float*)((int8_t*)workspace + rows * padded);
+        rc = hrf_quantize_rows_int8(x, x_type, rows, inner, ldx, (int8_t*)workspace, padded, scale, stream);
+        return rc ? rc : hrf_linear_int8((const int8_t*)workspace, padded, scale, w, ldw, w_scale, bias, rows, cols, padded, y, y_type, ldy, relu, stream);
+    }
+    I8Args A;
+    A.x = nullptr; A.w = w; A.sx = nullptr; A.sw = w_scale; A.bias = bias; A.y = y; A.ldx = 0; A.ldw = ldw; A.ldy = ldy;
+    A.rows = (int)rows; A.cols = (int)cols; A.inner = (int)padded; A.relu = relu;
+    if (x_type == I8_F32) i8_float<I8_F32>(A, x, ldx, inner, y_type, (hipStream_t)stream);
+    else if (x_type == I8_F16) i8_float<I8_F16>(A, x, ldx, inner, y_type, (hipStream_t)stream);
+    else i8_float<I8_BF16>(A, x, ldx, inner, y_type, (hipStream_t)stream);
     HRF_CHECK_LAUNCH();
     return 0;
 }

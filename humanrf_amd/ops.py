@@ -914,18 +914,19 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, x_scale: Optional[torch.Ten
     y = torch.empty(*x.shape[:-1], weight.out_features, dtype=out_dtype, device=x.device)
     if y.numel() == 0:
         return y
+    w, lib = weight.codes, _lib.lib()
     with _on_device(x.device), _span("linear_int8", m):
         if x_scale is None:
-            codes = torch.empty(m, int8_padded(k), dtype=torch.int8, device=x.device)
-            x_scale = torch.empty(m, dtype=torch.float32, device=x.device)
-            check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), _INT8_KINDS[x.dtype], m, k, rows.stride(0), ptr(codes), codes.shape[1],
-                                                    ptr(x_scale), stream_ptr()))
+            need = lib.hrf_linear_int8_workspace_bytes(m, weight.out_features, k)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            check(lib.hrf_linear_int8_float(ptr(rows), _INT8_KINDS[x.dtype], rows.stride(0), ptr(w), w.stride(0), ptr(weight.scale),
+                                            ptr(weight.bias), m, weight.out_features, k, ptr(y), _INT8_KINDS[out_dtype],
+                                            weight.out_features, 1 if relu else 0, ptr(ws), stream_ptr()))
         else:
             codes = _padded_int8(rows)
-        w = weight.codes
-        check(_lib.lib().hrf_linear_int8(ptr(codes), codes.stride(0), ptr(x_scale), ptr(w), w.stride(0), ptr(weight.scale), ptr(weight.bias),
-                                         m, weight.out_features, w.shape[1], ptr(y), _INT8_KINDS[out_dtype], weight.out_features,
-                                         1 if relu else 0, stream_ptr()))
+            check(lib.hrf_linear_int8(ptr(codes), codes.stride(0), ptr(x_scale), ptr(w), w.stride(0), ptr(weight.scale), ptr(weight.bias),
+                                      m, weight.out_features, w.shape[1], ptr(y), _INT8_KINDS[out_dtype], weight.out_features,
+                                      1 if relu else 0, stream_ptr()))
     return y
 
 

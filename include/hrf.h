@@ -575,6 +575,13 @@ int64_t hrf_int8_padded(int64_t cols);
 int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
                     const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
                     hrf_stream_t stream);
+/* The same with x in fp32, fp16 or bf16 (x_type 0, 1, 2; row stride ldx in values, `inner` its true length, any alignment): each row is
+ * rounded to 8 bits with a scale of its own, as hrf_quantize_rows_int8 does, then multiplied. w as above, its rows padded to
+ * hrf_int8_padded(inner). workspace: DEVICE scratch of hrf_linear_int8_workspace_bytes() bytes (may be 0), a multiple of 16 bytes. */
+int64_t hrf_linear_int8_workspace_bytes(int64_t rows, int64_t cols, int64_t inner);
+int hrf_linear_int8_float(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                          int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu, void* workspace,
+                          hrf_stream_t stream);
 /* Rows of x (x_type 0 fp32, 1 fp16, 2 bf16; row stride ldx) -> codes q (row stride ldq >= cols, filled with zeros behind cols) and one
  * scale a row: scale = a * (1 / 127), q = rint(x * (127 / a)), a = max(max |x|, 2^-119). A row that is not finite gets codes 0 and a
  * scale that is not finite. x_type 3: int8 rows are copied, with the padding (scale is not written and may be NULL). */

@@ -132,6 +132,22 @@ def test_rounding_rows_refuses(args):
     assert b"hrf_quantize_rows_int8" in lib.hrf_last_error()
 
 
+@pytest.mark.parametrize("change,said", [
+    (dict(x_type=3), b"x_type"), (dict(inner=0), b"sizes"), (dict(inner=131072), b"sizes"), (dict(x=None), b"NULL"), (dict(w=None), b"NULL"),
+    (dict(ldx=99), b"stride"), (dict(ldw=96), b"stride"), (dict(y_type=9), b"y_type"), (dict(workspace=None), b"workspace"),
+    (dict(workspace=FAKE + 8), b"workspace"), (dict(rows=-5), b"sizes"),
+])
+def test_the_product_of_float_rows_refuses(change, said):
+    from humanrf_amd import _lib
+    lib = _lib.lib()
+    a = dict(x=FAKE, x_type=2, ldx=100, w=FAKE, ldw=128, w_scale=FAKE, bias=None, rows=4, cols=8, inner=100, y=FAKE, y_type=0, ldy=8, relu=0,
+             workspace=FAKE, stream=None)
+    a.update(change)
+    assert lib.hrf_linear_int8_float(*a.values()) != 0
+    assert b"hrf_linear_int8_float" in lib.hrf_last_error() and said in lib.hrf_last_error()
+    assert lib.hrf_linear_int8_workspace_bytes(-1, 8, 100) == 0 and lib.hrf_linear_int8_workspace_bytes(4, 8, 100) >= 4 * (128 + 4)
+
+
 def test_padded_lengths():
     from humanrf_amd import _lib, ops
     lib = _lib.lib()
