@@ -108,8 +108,8 @@ _SIGNATURES = {
     "hrf_adam_multi": [_VP, _I32, _I32, _I64] + [_F] * 5 + [_VP, _VP, _VP, _VP],
     "hrf_adamw_multi": [_VP, _VP, _I32, _I32, _I32] + [_VP] * 5 + [_D, _VP] + [_D] * 6 + [_VP] * 3 + [ctypes.c_uint32, _I32, _VP],
     "hrf_grad_norm_multi": [_VP, _VP, _I32, _D] + [_VP] * 4,
-    "hrf_linear_int8": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I32, _I64, _I32, _VP],
-    "hrf_linear_int8_float": [_VP, _I32, _I64, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I32, _I64, _I32, _VP, _VP],
+    "hrf_linear_int8": [_VP, _I32, _I64, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _VP, _I32, _I64, _I32, _VP, _VP],
+    "hrf_int8_pack": [_VP, _I64, _I64, _I64, _VP, _VP],
     "hrf_quantize_rows_int8": [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _VP],
     "hrf_uniform_fill": [ctypes.c_uint32, _I64, _VP, _VP],
     "hrf_weights_fwd": [_VP] * 4 + [_I64, _VP, _VP],
@@ -137,6 +137,8 @@ def lib() -> ctypes.CDLL:
             l.hrf_adamw_workspace_bytes.argtypes = []
             l.hrf_int8_padded.restype = ctypes.c_int64
             l.hrf_int8_padded.argtypes = [_I64]
+            l.hrf_int8_packed_bytes.restype = ctypes.c_int64
+            l.hrf_int8_packed_bytes.argtypes = [_I64] * 2
             l.hrf_linear_int8_workspace_bytes.restype = ctypes.c_int64
             l.hrf_linear_int8_workspace_bytes.argtypes = [_I64] * 3
             l.hrf_scatter_workspace_bytes.restype = ctypes.c_size_t
@@ -157,7 +159,7 @@ def lib() -> ctypes.CDLL:
 
 def exported_symbols():
     """Names hrf.h declares (used by the CPU-side ABI test)."""
-    return ["hrf_last_error", "hrf_adam_workspace_bytes", "hrf_adamw_workspace_bytes", "hrf_int8_padded", "hrf_linear_int8_workspace_bytes", "hrf_scatter_workspace_bytes", "hrf_scatter_signals_per_segment",
+    return ["hrf_last_error", "hrf_adam_workspace_bytes", "hrf_adamw_workspace_bytes", "hrf_int8_padded", "hrf_int8_packed_bytes", "hrf_linear_int8_workspace_bytes", "hrf_scatter_workspace_bytes", "hrf_scatter_signals_per_segment",
             "hrf_can_stream_wait_value"] + list(_SIGNATURES.keys())
 
 

@@ -3,11 +3,15 @@
 //   y[m][n] = act( (sum_k xq[m][k] wq[n][k]) * sx[m] * sw[n] + bias[n] )        xq, wq in -128 .. 127, sums exact in int32
 //   row -> codes: s = amax * (1 / 127), q = rint(x * (127 / amax)), amax = max(max |x|, 2^-119)
 //
-// The sums are v_mfma_i32_16x16x64_i8: 16 bytes a lane and operand, row (lane & 15), bytes 16 (lane >> 4) .. + 15 of 64. The order of k
-// inside an instruction is the same for both operands, so it does not matter; the result's rows are W's channels, its columns x's tokens
-// (lane & 15), and a lane's four values are four consecutive channels of one token.
-// Rows of both operands begin at multiples of 16 bytes and are padded with zeros to a multiple of 64 (128 when longer than 64): a product
-// with padding is the product. Epilogue in fp32, one rounding per operation, one to the type of y.
+// The sums are v_mfma_i32_16x16x64_i8 and v_mfma_i32_32x32x32_i8: 16 bytes a lane and operand, row (lane & 15) or (lane & 31), a run of 16 k
+// for each lane further on. The order of k inside an instruction is the same for both operands, so it does not matter; W is the first
+// operand, so that a lane's results are neighbouring channels of one token.
+// W is packed: rows padded with zeros to 64 bytes (or a multiple of 128), cut into blocks of 16 rows x 64 bytes, a kilobyte
+// each, in which bytes 16 q .. 16 q + 15 of row t are the 16 bytes at 256 q + 16 t: what lane (t, q) of the first instruction takes. A
+// wavefront's load of an operand is then one kilobyte side by side. Few tokens are packed too; many stay rows, of which a stage of the
+// tiles reads 128 bytes each (rounding 8192 rows of 8192 straight into packed blocks takes 89 us, pieces of 16 bytes scattered by
+// different workgroups; into rows 35). 29 tokens x 10240 x 5120: both operands as rows, 16 pieces of 64 bytes a load, 31 us; packed 13.
+// Epilogue in fp32, one rounding per operation, one to the type of y.
 #include "hrf_common.h"
 #include <algorithm>
 
@@ -23,8 +27,11 @@ template <> struct I8Type<I8_F16> { typedef __half T; static __device__ float up
 template <> struct I8Type<I8_BF16> { typedef __bf16 T; static __device__ float up(__bf16 x) { return (float)x; } static __device__ __bf16 down(float x) { return (__bf16)x; } };
 
 // ------------------------------------------------------------------------------------------------ rows -> codes and scales
-// One 16-byte piece of a row, as fp32.
-template <int K> struct alignas(16) I8Piece { static constexpr int n = 16 / (int)sizeof(typename I8Type<K>::T); typename I8Type<K>::T v[16 / sizeof(typename I8Type<K>::T)]; };
+// 16 bytes of a row, at any address (unaligned accesses are the hardware's).
+template <int K> struct I8Piece { static constexpr int n = 16 / (int)sizeof(typename I8Type<K>::T); typename I8Type<K>::T v[16 / sizeof(typename I8Type<K>::T)]; };
+
+template <int K>
+__device__ __forceinline__ void i8_get(I8Piece<K>& v, const typename I8Type<K>::T* from) { __builtin_memcpy(&v, from, 16); }
 
 __device__ __forceinline__ uint32_t i8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }     // |x| as an integer: the order of the values, NaN on top
 
@@ -39,12 +46,18 @@ __device__ __forceinline__ float i8_factor(uint32_t top, float& scale)
 // Four values -> four codes in one word. |x| * factor is below 127.0001 (and 0 * NaN converts to 0), so that no clamp is needed.
 __device__ __forceinline__ uint32_t i8_code(float x, float factor, bool finite) { return finite ? (uint32_t)(int)rintf(x * factor) & 0xffu : 0u; }
 
-// kGroup lanes (a power of two, or the whole workgroup of 256 in groups of 64 joined through LDS) a row; the row is read once and stays in
-// registers, kPieces 16-byte pieces a lane. Both sides of that: rows of 4096 bf16 from memory twice, value by value, 118 us for 8192
-// of them; this way 35 us.
-template <int K, int kGroup, int kPieces>
+// Where code k of a row goes. Packed: see above. Otherwise rows of `ld` codes.
+template <bool kPacked>
+__device__ __forceinline__ int64_t i8_at(int64_t row, int k, int64_t ld)
+{
+    return kPacked ? ((row >> 4) * (ld >> 6) + (k >> 6)) * 1024 + ((k >> 4) & 3) * 256 + (row & 15) * 16 + (k & 15) : row * ld + k;
+}
+
+// kGroup lanes a row (a power of two up to a wavefront, or the whole workgroup of 256 joined through LDS). The row is read once, in 16-byte
+// pieces, and stays in registers, kPieces of them a lane. 8192 rows of 8192 bf16: 118 us read twice value by value, 35 us this way.
+template <int K, bool kPacked, int kGroup, int kPieces>
 __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>::T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
-                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
+                                                            int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
 {
     __shared__ uint32_t s_max[4];
     constexpr int n = I8Piece<K>::n, kRows = 256 / kGroup;
@@ -57,7 +70,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
         const int k0 = (p * kGroup + lane) * n;
-        if (k0 + n <= cols) v[p] = *(const I8Piece<K>*)(from + k0);
+        if (k0 + n <= cols) i8_get<K>(v[p], from + k0);
         else {
 #pragma unroll
             for (int k = 0; k < n; ++k) v[p].v[k] = k0 + k < cols ? from[k0 + k] : I8Type<K>::down(0.0f);
@@ -79,11 +92,10 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
     const float factor = i8_factor(top, sc);
     const bool finite = top < 0x7f800000u;
     if (lane == 0) scale[row] = sc;
-    int8_t* const to = q + row * ldq;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
         const int k0 = (p * kGroup + lane) * n;
-        if (k0 >= ldq) continue;        // (the padding up to ldq is a multiple of 64 away: whole pieces)
+        if (k0 >= ldq) continue;        // (ldq is a multiple of 8: whole pieces)
         uint32_t word[n / 4];
 #pragma unroll
         for (int w = 0; w < n / 4; ++w) {
@@ -91,19 +103,19 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
 #pragma unroll
             for (int k = 0; k < 4; ++k) word[w] |= i8_code(I8Type<K>::up(v[p].v[4 * w + k]), factor, finite) << (8 * k);
         }
-        if (n == 8) *(uint2*)(to + k0) = make_uint2(word[0], word[n / 4 - 1]);
-        else *(uint32_t*)(to + k0) = word[0];
+        int8_t* const to = q + i8_at<kPacked>(row, k0, ldq);
+        if (n == 8) *(uint2*)to = make_uint2(word[0], word[n / 4 - 1]);
+        else *(uint32_t*)to = word[0];
     }
 }
 
-// Rows at addresses that are no multiples of 16 bytes, or longer than 16384: value by value, twice.
-template <int K>
+// Codes that do not begin at multiples of 8 bytes, and rows too long for the registers: value by value, twice.
+template <int K, bool kPacked>
 __global__ __launch_bounds__(256) void k_quantize_rows_any(const typename I8Type<K>::T* __restrict__ x, int64_t cols, int64_t ldx,
                                                            int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
 {
     __shared__ uint32_t s_max[4];
     x += (int64_t)blockIdx.x * ldx;
-    q += (int64_t)blockIdx.x * ldq;
     uint32_t top = 0;
     for (int64_t k = threadIdx.x; k < cols; k += 256) top = max(top, i8_bits(I8Type<K>::up(x[k])));
 #pragma unroll
@@ -115,25 +127,57 @@ __global__ __launch_bounds__(256) void k_quantize_rows_any(const typename I8Type
     const float factor = i8_factor(top, sc);
     const bool finite = top < 0x7f800000u;
     if (threadIdx.x == 0) scale[blockIdx.x] = sc;
-    for (int64_t k = threadIdx.x; k < ldq; k += 256) q[k] = k < cols ? (int8_t)i8_code(I8Type<K>::up(x[k]), factor, finite) : (int8_t)0;
+    for (int k = threadIdx.x; k < (int)ldq; k += 256)
+        q[i8_at<kPacked>(blockIdx.x, k, ldq)] = k < cols ? (int8_t)i8_code(I8Type<K>::up(x[k]), factor, finite) : (int8_t)0;
 }
 
-__global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, int64_t cols, int64_t ldx, int8_t* __restrict__ q, int64_t ldq)
+// Rows of codes -> rows padded with zeros to ldq, a multiple of 16 bytes.
+__global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, int cols, int64_t ldx, int8_t* __restrict__ q, int ldq)
 {
     x += (int64_t)blockIdx.x * ldx;
     q += (int64_t)blockIdx.x * ldq;
-    for (int64_t k = threadIdx.x; k < ldq; k += 256) q[k] = k < cols ? x[k] : (int8_t)0;
+    for (int k0 = threadIdx.x * 16; k0 < ldq; k0 += 4096) {
+        i8_v4 v = {0, 0, 0, 0};
+        if (k0 + 16 <= cols) __builtin_memcpy(&v, x + k0, 16);
+        else
+            for (int k = 0; k0 + k < cols; ++k) v[k >> 2] |= (int)((uint32_t)(uint8_t)x[k0 + k] << (8 * (k & 3)));
+        *(i8_v4*)(q + k0) = v;
+    }
+}
+
+// Rows of codes -> packed, a thread for each 16 bytes of the result; rows up to the next multiple of 16 are zeros.
+__global__ __launch_bounds__(256) void k_pack_rows(const int8_t* __restrict__ x, int64_t rows, int cols, int64_t ldx,
+                                                   int8_t* __restrict__ packed, int64_t padded, int64_t pieces)
+{
+    const int64_t piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (piece >= pieces) return;
+    const int64_t block = piece >> 6, runs = padded >> 6, row = block / runs * 16 + (piece & 15);
+    const int k0 = (int)(block % runs) * 64 + ((int)(piece >> 4) & 3) * 16;
+    i8_v4 v = {0, 0, 0, 0};
+    if (row < rows) {
+        const int8_t* from = x + row * ldx + k0;
+        if (k0 + 16 <= cols) __builtin_memcpy(&v, from, 16);
+        else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k0 + 4 * w + k < cols) v[w] |= (int)((uint32_t)(uint8_t)from[4 * w + k] << (8 * k));
+        }
+    }
+    ((i8_v4*)packed)[piece] = v;
 }
 
 // ------------------------------------------------------------------------------------------------ product
 struct I8Args {
-    const int8_t* x;
-    const int8_t* w;
+    const int8_t* x;            // codes: packed for few tokens, else rows of ldx bytes
+    int64_t ldx;
+    const int8_t* w;            // packed
     const float* sx;
     const float* sw;
     const float* bias;
     void* y;
-    int64_t ldx, ldw, ldy;
+    int64_t ldy;
     int rows, cols, inner;      // inner: padded
     int relu;
 };
@@ -145,6 +189,24 @@ __device__ __forceinline__ typename I8Type<K>::T i8_finish(int acc, float sx, fl
     if (has_bias) v = v + bias;
     if (relu) v = v < 0.0f ? 0.0f : v;
     return I8Type<K>::down(v);
+}
+
+// N neighbouring values, 16 bytes, of a row of y from column n on.
+template <typename T, int N>
+__device__ __forceinline__ void i8_store(T* row, int n, int cols, bool here, const T* v)
+{
+    static_assert(N * sizeof(T) == 16, "a piece is 16 bytes");
+    if (!here) return;
+    if (n + N <= cols) {
+        i8_v4 piece;
+        __builtin_memcpy(&piece, v, 16);
+        asm("" : "+v"(piece));      // (a whole piece: left alone, the last value's store is shared with the other branch)
+        __builtin_memcpy(row + n, &piece, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (n + k < cols) row[n + k] = v[k];
+    }
 }
 
 // 16 bytes from base + offset (each lane its own) to LDS, the wavefront's kilobyte from byte `to` on in the order of its lanes. The
@@ -167,10 +229,13 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 }
 
 // Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 128
-// bytes of k in LDS, two stages, filled by direct loads (16 bytes a lane, no registers). A row's eight 16-byte chunks lie in LDS permuted
-// by its number, so that lanes that read the same chunk of neighbouring rows hit all banks.
+// bytes of k in LDS, two stages, filled by direct loads (16 bytes a lane, no registers). W's packed blocks lie there as in memory: 16
+// lanes that read together read 256 bytes side by side. A token's eight 16-byte chunks lie permuted by its number, so that lanes that
+// read the same chunk of neighbouring tokens hit all banks.
 // The operands of the next 32 k are read from LDS while the matrix cores work on these; before the last 32 k of a stage the workgroup
 // meets, the loads of the stage after the next take the buffer that everybody has read, and the next stage's first operands follow.
+// LDS is what bounds smaller tiles: it gives 128 bytes a clock, and 128 x 128 tiles ask for 187 where 256 x 256 ask for 94. 8192^3:
+// 897 us with 128 x 128 tiles, 540 us (2.04 POP/s) with 256 x 256; the library's product of the same integers reaches 2.14.
 template <int K, int TM, int TN>
 __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const I8Args A)
 {
@@ -183,22 +248,19 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
     int tm, tn;
     i8_tile_of((A.rows + BM - 1) / BM, (A.cols + BN - 1) / BN, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int8_t* const xb = A.x + (int64_t)m0 * A.ldx;
-    const int8_t* const wb = A.w + (int64_t)n0 * A.ldw;
     const int steps = A.inner >> 7;
 
-    // this lane's part of each load: row first + lane / 8 of the stage (rows past the end read the last one), its chunk permuted
+    // Load i of the wavefronts 0, 1: eight tokens, this lane's row first + lane / 8 (past the end: the last one), its chunk permuted.
+    // Of the wavefronts 2, 3: half a stage of 16 channels, a block (past the end: the last one).
     uint32_t from[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int first = (wave * kLoads + i) * 8, r = first + (lane >> 3), chunk = (lane & 7) ^ ((lane >> 3) & 7);
-        from[i] = (first < BM ? (uint32_t)min(r, A.rows - 1 - m0) * (uint32_t)A.ldx : (uint32_t)min(r - BM, A.cols - 1 - n0) * (uint32_t)A.ldw) + chunk * 16;
-    }
-    const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile;
-    auto load = [&](int i, int buf, int k0) {
-        const int first = (wave * kLoads + i) * 8;
-        i8_load_lds((first < BM ? xb : wb) + k0, from[i], lds + buf * kStage + first * 128);
-    };
+    for (int i = 0; i < kLoads; ++i)
+        from[i] = wave < 2 ? (uint32_t)min((wave * kLoads + i) * 8 + (lane >> 3), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 7) ^ (lane >> 3)) * 16
+                           : (uint32_t)(min((n0 >> 4) + ((wave - 2) * kLoads + i) / 2, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + (i & 1) * 1024 + lane * 16;
+    const int8_t* const base = wave < 2 ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
+    const int forward = wave < 2 ? 128 : 2048;
+    const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kLoads * 1024;
+    auto load = [&](int i, int buf, int s) { i8_load_lds(base + (int64_t)s * forward, from[i], lds + buf * kStage + i * 1024); };
     i8_v16 acc[TN][TM];
 #pragma unroll
     for (int a = 0; a < TN; ++a)
@@ -207,14 +269,15 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[a][b][k] = 0;
     i8_v4 fx[2][TM], fw[2][TN];
-    const int x_row = (wm * 32 * TM + (lane & 31)) * 128, w_row = (BM + wn * 32 * TN + (lane & 31)) * 128;
+    const int x_row = (wm * 32 * TM + (lane & 31)) * 128;
+    const int w_row = (BM / 16 + wn * 2 * TN) * 2048 + ((lane >> 4) & 1) * 2048 + (lane >> 5) * 256 + (lane & 15) * 16;
     auto read = [&](int set, int buf, int kk) {
+        const int8_t* t = s_tile + buf * kStage;
         const int chunk = ((kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16;
-        const int8_t* t = s_tile + buf * kStage + chunk;
 #pragma unroll
-        for (int b = 0; b < TM; ++b) fx[set][b] = *(const i8_v4*)(t + x_row + b * 32 * 128);
+        for (int b = 0; b < TM; ++b) fx[set][b] = *(const i8_v4*)(t + x_row + chunk + b * 4096);
 #pragma unroll
-        for (int a = 0; a < TN; ++a) fw[set][a] = *(const i8_v4*)(t + w_row + a * 32 * 128);
+        for (int a = 0; a < TN; ++a) fw[set][a] = *(const i8_v4*)(t + w_row + kk * 512 + a * 4096);
     };
     auto multiply = [&](int set) {
 #pragma unroll
@@ -233,72 +296,78 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (steps > 1) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(i, 1, 128);
+        for (int i = 0; i < kLoads; ++i) load(i, 1, 1);
     }
     read(0, 0, 0);
-    for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
+    auto three = [&](int buf) {
 #pragma unroll
         for (int kk = 0; kk < 3; ++kk) {
             read((kk + 1) & 1, buf, kk + 1);
             multiply(kk & 1);
-#ifndef NO_SGB
 #pragma unroll
             for (int i = 0; i < TM + TN; ++i) {     // one operand read for every TM TN / (TM + TN) products
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, TM * TN / (TM + TN), 0);
             }
-#endif
         }
+    };
+    for (int s = 0; s + 1 < steps; ++s) {
+        const int buf = s & 1;
+        three(buf);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");     // the next stage has landed, this one is in registers
-        if (s + 1 < steps) read(0, buf ^ 1, 0);
+        read(0, buf ^ 1, 0);
         if (s + 2 < steps) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) load(i, buf, (s + 2) << 7);
+            for (int i = 0; i < kLoads; ++i) load(i, buf, s + 2);
         }
         multiply(1);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-
-    // Epilogue: through LDS, so that a row of y leaves in 16-byte pieces side by side. Pieces lie permuted by their row's number again.
-    constexpr int kPer = 16 / (int)sizeof(T), kPieces = BN / kPer;          // values a piece, pieces a row
-    constexpr int kPasses = BM * BN * (int)sizeof(T) > 2 * kStage ? 2 : 1, kRows = BM / kPasses;
-    T* const out = (T*)s_tile;
+    three((steps - 1) & 1);
+    multiply(1);
+    // Epilogue, 32 channels of 32 tokens at a time: a lane holds channels 8 g + 4 (lane / 32) + 0 .. 3 of token lane % 32. For 16-bit y the
+    // halves of the wavefront trade, so that a lane has eight neighbouring channels, 16 bytes. (Through LDS, whole rows at a time, this
+    // took as long as 2000 k of products: there is no other workgroup on the CU to work meanwhile.)
     const bool has_bias = A.bias != nullptr, relu = A.relu != 0;
-    const bool wide = (((uintptr_t)A.y | (uintptr_t)(A.ldy * (int64_t)sizeof(T))) & 15u) == 0;
 #pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-        if (kPasses == 1 || wm == pass) {
+    for (int a = 0; a < TN; ++a) {
+        const int nl = wn * 32 * TN + a * 32 + (lane >> 5) * 4;
+        float sw[16], bias[16];
 #pragma unroll
-            for (int b = 0; b < TM; ++b) {
-                const int ml = wm * 32 * TM + b * 32 + (lane & 31), row = ml - pass * kRows;
-                const float sx = s_sx[ml];
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-                for (int a = 0; a < TN; ++a)
+            for (int k = 0; k < 4; ++k) {
+                sw[g * 4 + k] = s_sw[nl + g * 8 + k];
+                bias[g * 4 + k] = s_bias[nl + g * 8 + k];
+            }
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int nl = wn * 32 * TN + a * 32 + g * 8 + (lane >> 5) * 4;
-                        T v[4];
+        for (int b = 0; b < TM; ++b) {
+            const int ml = wm * 32 * TM + b * 32 + (lane & 31), m = m0 + ml;
+            const float sx = s_sx[ml];
+            T v[16];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = i8_finish<K>(acc[a][b][g * 4 + k], sx, s_sw[nl + k], s_bias[nl + k], has_bias, relu);
-                        T* to = out + row * BN + ((nl / kPer) ^ (row & (kPieces - 1))) * kPer + nl % kPer;
-                        if (sizeof(T) == 4) *(i8_v4*)to = *(const i8_v4*)v;
-                        else *(uint64_t*)to = *(const uint64_t*)v;
+            for (int k = 0; k < 16; ++k) v[k] = i8_finish<K>(acc[a][b][k], sx, sw[k], bias[k], has_bias, relu);
+            T* const y = (T*)A.y + (int64_t)m * A.ldy;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) i8_store<T, 4>(y, n0 + nl + g * 8, A.cols, m < A.rows, v + g * 4);
+            } else {
+#pragma unroll
+                for (int g = 0; g < 4; g += 2) {
+                    uint32_t u[4];
+                    __builtin_memcpy(u, v + g * 4, 16);         // this lane's four of g, four of g + 1
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {               // lower half: all of g, upper half: all of g + 1
+                        const auto both = __builtin_amdgcn_permlane32_swap(u[h], u[2 + h], false, false);
+                        u[h] = both[0];
+                        u[2 + h] = both[1];
                     }
+                    T eight[8];
+                    __builtin_memcpy(eight, u, 16);
+                    i8_store<T, 8>(y, n0 + wn * 32 * TN + a * 32 + (g + (lane >> 5)) * 8, A.cols, m < A.rows, eight);
+                }
             }
         }
-        __syncthreads();
-        for (int p = threadIdx.x; p < kRows * kPieces; p += 256) {
-            const int row = p / kPieces, piece = p % kPieces;
-            const int m = m0 + pass * kRows + row, n = n0 + piece * kPer;
-            if (m >= A.rows || n >= A.cols) continue;
-            const T* v = out + row * BN + (piece ^ (row & (kPieces - 1))) * kPer;
-            T* y = (T*)A.y + (int64_t)m * A.ldy + n;
-            if (wide && n + kPer <= A.cols) *(i8_v4*)y = *(const i8_v4*)v;
-            else
-                for (int k = 0; k < kPer && n + k < A.cols; ++k) y[k] = v[k];
-        }
-        if (pass + 1 < kPasses) __syncthreads();
+        asm volatile("" ::: "memory");      // (one a at a time: the compiler would fetch all the scales first, and spill)
     }
 }
 
@@ -308,10 +377,10 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
 // channels are dealt to the instructions so that a lane's 16 results are 16 neighbouring channels of one token: 32 bytes of fp16 in a
 // row of 128.
 struct I8Short {
-    const void* x;
+    const void* x;          // rows as the caller has them
     int64_t ldx;
+    const float* sx;        // of integer rows
     int inner;              // not padded
-    int x_wide, y_wide;     // rows of x / y begin at multiples of 16 bytes
 };
 
 template <int X, int K, int KS>
@@ -326,9 +395,10 @@ __global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A, const I
     float sw[16], bias[16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-        const int row = min(n0 + (t >> 2) * 16 + a * 4 + (t & 3), A.cols - 1);
+        // row a * 4 + t % 4 of the block of 16 that t / 4 names (past the last one: the last again)
+        const int64_t block = min((n0 >> 4) + (t >> 2), (A.cols - 1) >> 4);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) fw[s][a] = *(const i8_v4*)(A.w + (int64_t)row * A.ldw + s * 64 + q * 16);
+        for (int s = 0; s < KS; ++s) fw[s][a] = *(const i8_v4*)(A.w + (block * KS + s) * 1024 + q * 256 + (a * 4 + (t & 3)) * 16);
     }
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
@@ -344,8 +414,21 @@ __global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A, const I
         float sx;
         if constexpr (X == I8_INT8) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) fx[s] = *(const i8_v4*)((const int8_t*)B.x + row * B.ldx + s * 64 + q * 16);
-            sx = A.sx[row];
+            for (int s = 0; s < KS; ++s) {
+                const int8_t* const from = (const int8_t*)B.x + row * B.ldx;
+                const int k0 = s * 64 + q * 16;
+                if (k0 + 16 <= B.inner) __builtin_memcpy(&fx[s], from + k0, 16);
+                else {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        fx[s][w] = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k0 + 4 * w + k < B.inner) fx[s][w] |= (int)((uint32_t)(uint8_t)from[k0 + 4 * w + k] << (8 * k));
+                    }
+                }
+            }
+            sx = B.sx[row];
         } else {
             typedef typename I8Type<X>::T XT;
             constexpr int n = I8Piece<X>::n, kPieces = 16 / n;
@@ -357,7 +440,7 @@ __global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A, const I
 #pragma unroll
                 for (int p = 0; p < kPieces; ++p) {
                     const int k0 = s * 64 + q * 16 + p * n;
-                    if (B.x_wide && k0 + n <= B.inner) v[s][p] = *(const I8Piece<X>*)(from + k0);
+                    if (k0 + n <= B.inner) i8_get<X>(v[s][p], from + k0);
                     else {
 #pragma unroll
                         for (int k = 0; k < n; ++k) v[s][p].v[k] = k0 + k < B.inner ? from[k0 + k] : I8Type<X>::down(0.0f);
@@ -392,17 +475,9 @@ __global__ __launch_bounds__(256) void k_linear_i8_short(const I8Args A, const I
 #pragma unroll
             for (int k = 0; k < 4; ++k) out[a * 4 + k] = i8_finish<K>(acc[k], sx, sw[a * 4 + k], bias[a * 4 + k], has_bias, relu);
         }
-        if (m >= A.rows) continue;
-        const int n = n0 + q * 16;
-        T* const y = (T*)A.y + row * A.ldy + n;
-        if (B.y_wide && n + 16 <= A.cols) {
+        constexpr int n = 16 / (int)sizeof(T);
 #pragma unroll
-            for (int p = 0; p < (int)sizeof(T); ++p) ((i8_v4*)y)[p] = ((const i8_v4*)out)[p];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-                if (n + k < A.cols) y[k] = out[k];
-        }
+        for (int p = 0; p < 16 / n; ++p) i8_store<T, n>((T*)A.y + row * A.ldy, n0 + q * 16 + p * n, A.cols, m < A.rows, out + p * n);
     }
 }
 
@@ -413,15 +488,15 @@ __global__ __launch_bounds__(64 * kWaves) void k_linear_i8_few(const I8Args A)
 {
     typedef typename I8Type<K>::T T;
     __shared__ i8_v4 s_part[kWaves][MT * NT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n0 = (int)blockIdx.x * 16 * NT;
     const int runs = A.inner >> 6, each = (runs + kWaves - 1) / kWaves, begin = wave * each, end = min(begin + each, runs);
     const int8_t* w[NT];
     const int8_t* x[MT];
 #pragma unroll
-    for (int a = 0; a < NT; ++a) w[a] = A.w + (int64_t)min(n0 + a * 16 + t, A.cols - 1) * A.ldw + q * 16;
+    for (int a = 0; a < NT; ++a) w[a] = A.w + (int64_t)min((n0 >> 4) + a, (A.cols - 1) >> 4) * runs * 1024 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < MT; ++b) x[b] = A.x + (int64_t)min(b * 16 + t, A.rows - 1) * A.ldx + q * 16;
+    for (int b = 0; b < MT; ++b) x[b] = A.x + (int64_t)min(b, (A.rows - 1) >> 4) * runs * 1024 + lane * 16;
     i8_v4 acc[NT][MT];
 #pragma unroll
     for (int a = 0; a < NT; ++a)
@@ -432,9 +507,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_linear_i8_few(const I8Args A)
         i8_v4 fw[kAhead][NT], fx[kAhead][MT];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int64_t k = (int64_t)min(r + u, end - 1) * 64;
+            const int64_t k = (int64_t)min(r + u, end - 1) * 1024;
 #pragma unroll
-            for (int a = 0; a < NT; ++a) fw[u][a] = __builtin_nontemporal_load((const i8_v4*)(w[a] + k));
+            for (int a = 0; a < NT; ++a) fw[u][a] = *(const i8_v4*)(w[a] + k);
 #pragma unroll
             for (int b = 0; b < MT; ++b) fx[u][b] = *(const i8_v4*)(x[b] + k);
         }
@@ -463,59 +538,51 @@ __global__ __launch_bounds__(64 * kWaves) void k_linear_i8_few(const I8Args A)
     }
 }
 
-template <int K>
+static int i8_padded(int64_t cols) { return (int)(cols <= 64 ? 64 : (cols + 127) / 128 * 128); }
+
+// ldq: row stride of the codes, or their padded length when they are packed
+template <int K, bool kPacked>
 static void i8_quantize(const void* xv, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, hipStream_t stream)
 {
     typedef typename I8Type<K>::T T;
     const T* x = (const T*)xv;
     constexpr int n = I8Piece<K>::n;
-    const int64_t width = std::max(cols, ldq);
-    // whole pieces: rows of x at multiples of 16 bytes, rows of q at multiples of 8 and padded to them
-    const bool pieces = (((uintptr_t)x | (uintptr_t)(ldx * (int64_t)sizeof(T))) & 15u) == 0 && (((uintptr_t)q | (uintptr_t)ldq) & 7u) == 0;
-#define I8_ROWS(G, P)                                                                                                            \
-    hipLaunchKernelGGL((k_quantize_rows<K, G, P>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))), dim3(256), 0, stream, x, rows, \
+    const bool pieces = (((uintptr_t)q | (uintptr_t)ldq) & 7u) == 0;
+#define I8_ROWS(G, P)                                                                                                                  \
+    hipLaunchKernelGGL((k_quantize_rows<K, kPacked, G, P>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))), dim3(256), 0, stream, x, rows, \
                        (int)cols, ldx, q, ldq, scale)
-    if (!pieces || width > 256 * 8 * n)
-        hipLaunchKernelGGL(k_quantize_rows_any<K>, dim3((unsigned)rows), dim3(256), 0, stream, x, cols, ldx, q, ldq, scale);
-    else if (width <= 16 * n) I8_ROWS(16, 1);
-    else if (width <= 64 * n) I8_ROWS(64, 1);
-    else if (width <= 64 * 4 * n) I8_ROWS(64, 4);
-    else if (width <= 256 * 4 * n) I8_ROWS(256, 4);
+    if (!pieces || ldq > 256 * 8 * n)
+        hipLaunchKernelGGL((k_quantize_rows_any<K, kPacked>), dim3((unsigned)rows), dim3(256), 0, stream, x, cols, ldx, q, ldq, scale);
+    else if (ldq <= 16 * n) I8_ROWS(16, 1);
+    else if (ldq <= 64 * n) I8_ROWS(64, 1);
+    else if (ldq <= 64 * 4 * n && !kPacked) I8_ROWS(64, 4);
+    else if (ldq <= 256 * 2 * n) I8_ROWS(256, 2);
+    else if (ldq <= 256 * 4 * n) I8_ROWS(256, 4);
     else I8_ROWS(256, 8);
 #undef I8_ROWS
 }
 
-static int i8_padded(int64_t cols) { return (int)(cols <= 64 ? 64 : (cols + 127) / 128 * 128); }
-
-extern "C" int64_t hrf_int8_padded(int64_t cols) { return cols < 1 || cols > HRF_INT8_MAX_INNER ? -1 : i8_padded(cols); }
-
-extern "C" int hrf_quantize_rows_int8(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
-                                      float* scale, hrf_stream_t stream)
+template <bool kPacked>
+static void i8_rows(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, hipStream_t stream)
 {
-    HRF_CHECK_ARG(x_type >= I8_F32 && x_type <= I8_INT8, "x_type must be 0 (fp32), 1 (fp16), 2 (bf16) or 3 (int8)");
-    HRF_CHECK_ARG(rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols <= HRF_INT8_MAX_INNER, "bad sizes");
-    if (rows == 0) return 0;
-    HRF_CHECK_ARG(x && q && (scale || x_type == I8_INT8), "NULL argument");
-    HRF_CHECK_ARG((ldx >= cols || rows == 1) && ldq >= cols, "a row stride is shorter than the row");
-    if (x_type == I8_F32) i8_quantize<I8_F32>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
-    else if (x_type == I8_F16) i8_quantize<I8_F16>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
-    else if (x_type == I8_BF16) i8_quantize<I8_BF16>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
-    else hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const int8_t*)x, cols, ldx, q, ldq);
-    HRF_CHECK_LAUNCH();
-    return 0;
+    if (x_type == I8_F32) i8_quantize<I8_F32, kPacked>(x, rows, cols, ldx, q, ldq, scale, stream);
+    else if (x_type == I8_F16) i8_quantize<I8_F16, kPacked>(x, rows, cols, ldx, q, ldq, scale, stream);
+    else i8_quantize<I8_BF16, kPacked>(x, rows, cols, ldx, q, ldq, scale, stream);
 }
 
-static bool i8_wide(const void* p, int64_t ld, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & 15u) == 0; }
+static void i8_pack(const int8_t* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* packed, hipStream_t stream)
+{
+    const int64_t padded = i8_padded(cols), pieces = (rows + 15) / 16 * padded;
+    hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, x, rows, (int)cols, ldx, packed, padded, pieces);
+}
 
 // Rows of up to 256 values and up to 128 channels, when there are enough rows to fill the card.
-static bool i8_is_short(int64_t rows, int64_t cols, int64_t inner) { return inner == 64 || (inner <= 256 && cols <= 128 && rows > 4096); }
+static bool i8_is_short(int64_t rows, int64_t cols, int64_t padded) { return padded == 64 || (padded <= 256 && cols <= 128 && rows > 4096); }
 
 template <int X, int K>
-static void i8_short(const I8Args& A, const void* x, int64_t ldx, int64_t inner, int size, hipStream_t stream)
+static void i8_short(const I8Args& A, const I8Short& B, hipStream_t stream)
 {
-    I8Short B;
-    B.x = x; B.ldx = ldx; B.inner = (int)inner; B.x_wide = i8_wide(x, ldx, size); B.y_wide = i8_wide(A.y, A.ldy, (int)sizeof(typename I8Type<K>::T));
-    const dim3 grid((unsigned)std::min<int64_t>((A.rows + 63) / 64, 2048), (unsigned)((A.cols + 63) / 64));
+    const dim3 grid((unsigned)std::min<int64_t>(((int64_t)A.rows + 63) / 64, 2048), (unsigned)((A.cols + 63) / 64));
     if (A.inner == 64) hipLaunchKernelGGL((k_linear_i8_short<X, K, 1>), grid, dim3(256), 0, stream, A, B);
     else if (A.inner == 128) hipLaunchKernelGGL((k_linear_i8_short<X, K, 2>), grid, dim3(256), 0, stream, A, B);
     else hipLaunchKernelGGL((k_linear_i8_short<X, K, 4>), grid, dim3(256), 0, stream, A, B);
@@ -529,13 +596,14 @@ static void i8_few(const I8Args& A, hipStream_t stream)
     else hipLaunchKernelGGL((k_linear_i8_few<K, MT, NT, 4>), grid, dim3(256), 0, stream, A);
 }
 
+#define I8_FEW 64       // rows up to which the product of few tokens runs, on packed codes
+
 template <int K>
 static void i8_linear(const I8Args& A, hipStream_t stream)
 {
-    if (i8_is_short(A.rows, A.cols, A.inner)) { i8_short<I8_INT8, K>(A, A.x, A.ldx, A.inner, 1, stream); return; }
     if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
     if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
-    if (A.rows <= 64) { i8_few<K, 4, 2>(A, stream); return; }
+    if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return; }
     const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256);
     if (large >= 200) hipLaunchKernelGGL((k_linear_i8<K, 4, 4>), dim3((unsigned)large), dim3(256), 0, stream, A);
     else {
@@ -544,82 +612,95 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     }
 }
 
-#define I8_CHECK(cond, msg)                      \
-    do {                                         \
-        if (!(cond)) {                           \
-            hrf_set_error("%s: %s", name, msg);  \
-            return 1;                            \
-        }                                        \
-    } while (0)
-static int i8_check(const char* name, const void* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
-                    int64_t rows, int64_t cols, int64_t inner, const void* y, int y_type, int64_t ldy)
+template <int K>
+static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const float* x_scale, int inner, void* workspace, hipStream_t stream)
 {
-    I8_CHECK(y_type >= I8_F32 && y_type <= I8_BF16, "y_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
-    I8_CHECK(rows >= 0 && rows < ((int64_t)1 << 31) - 256 && cols >= 0 && cols < ((int64_t)1 << 31) - 256, "bad sizes");
-    I8_CHECK(inner >= 64 && inner <= HRF_INT8_MAX_INNER + 1 && inner == i8_padded(inner), "inner must be a padded length (hrf_int8_padded)");
-    if (rows == 0 || cols == 0) return 0;
-    I8_CHECK(x && x_scale && w && w_scale && y, "NULL argument");
-    I8_CHECK((ldx >= inner || rows == 1) && (ldw >= inner || cols == 1) && (ldy >= cols || rows == 1), "a row stride is shorter than the row");
-    I8_CHECK((((uintptr_t)x | (uintptr_t)w) & 15u) == 0 && ((ldx | ldw) & 15) == 0, "x and w and their rows must begin at multiples of 16 bytes");
-    I8_CHECK(ldx < HRF_INT8_MAX_STRIDE && ldw < HRF_INT8_MAX_STRIDE, "rows are too far apart");
-    I8_CHECK(((rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 31) && cols <= 64 * 65535, "too many tiles");
-    return 0;
+    if (i8_is_short(A.rows, A.cols, A.inner)) {
+        I8Short B;
+        B.x = x; B.ldx = ldx; B.sx = x_scale; B.inner = inner;
+        if (x_type == I8_F32) i8_short<I8_F32, K>(A, B, stream);
+        else if (x_type == I8_F16) i8_short<I8_F16, K>(A, B, stream);
+        else if (x_type == I8_BF16) i8_short<I8_BF16, K>(A, B, stream);
+        else i8_short<I8_INT8, K>(A, B, stream);
+        return;
+    }
+    float* const scale = (float*)((int8_t*)workspace + ((int64_t)A.rows + 15) / 16 * 16 * A.inner);
+    A.x = (const int8_t*)workspace;
+    A.ldx = A.inner;
+    A.sx = x_type == I8_INT8 ? x_scale : scale;
+    const bool few = A.rows <= I8_FEW;
+    if (x_type != I8_INT8) {
+        if (few) i8_rows<true>(x, x_type, A.rows, inner, ldx, (int8_t*)workspace, A.inner, scale, stream);
+        else i8_rows<false>(x, x_type, A.rows, inner, ldx, (int8_t*)workspace, A.inner, scale, stream);
+    } else if (few) {
+        i8_pack((const int8_t*)x, A.rows, inner, ldx, (int8_t*)workspace, stream);
+    } else if (inner == A.inner && (((uintptr_t)x | (uintptr_t)ldx) & 15u) == 0 && ldx < (1 << 23)) {
+        A.x = (const int8_t*)x;         // rows that lie as the tiles read them
+        A.ldx = ldx;
+    } else {
+        hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)A.rows), dim3(256), 0, stream, (const int8_t*)x, inner, ldx, (int8_t*)workspace, A.inner);
+    }
+    i8_linear<K>(A, stream);
 }
 
-extern "C" int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
-                               const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
-                               hrf_stream_t stream)
+static bool i8_inner_ok(int64_t inner) { return inner >= 1 && inner <= HRF_INT8_MAX_INNER; }
+
+extern "C" int64_t hrf_int8_padded(int64_t inner) { return i8_inner_ok(inner) ? i8_padded(inner) : -1; }
+
+extern "C" int64_t hrf_int8_packed_bytes(int64_t rows, int64_t inner) { return rows < 0 || !i8_inner_ok(inner) ? -1 : (rows + 15) / 16 * 16 * i8_padded(inner); }
+
+extern "C" int64_t hrf_linear_int8_workspace_bytes(int64_t rows, int64_t cols, int64_t inner)
 {
-    const int rc = i8_check(__func__, x, ldx, x_scale, w, ldw, w_scale, rows, cols, inner, y, y_type, ldy);
-    if (rc || rows == 0 || cols == 0) return rc;
-    I8Args A;
-    A.x = x; A.w = w; A.sx = x_scale; A.sw = w_scale; A.bias = bias; A.y = y; A.ldx = ldx; A.ldw = ldw; A.ldy = ldy;
-    A.rows = (int)rows; A.cols = (int)cols; A.inner = (int)inner; A.relu = relu;
-    if (y_type == I8_F32) i8_linear<I8_F32>(A, (hipStream_t)stream);
-    else if (y_type == I8_F16) i8_linear<I8_F16>(A, (hipStream_t)stream);
-    else i8_linear<I8_BF16>(A, (hipStream_t)stream);
+    if (rows <= 0 || cols <= 0 || !i8_inner_ok(inner) || i8_is_short(rows, cols, i8_padded(inner))) return 0;
+    return hrf_int8_packed_bytes(rows, inner) + rows * 4;
+}
+
+extern "C" int hrf_quantize_rows_int8(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                                      float* scale, hrf_stream_t stream)
+{
+    HRF_CHECK_ARG(x_type >= I8_F32 && x_type <= I8_BF16, "x_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    HRF_CHECK_ARG(rows >= 0 && rows < HRF_INT8_MAX_ROWS && i8_inner_ok(cols), "bad sizes");
+    if (rows == 0) return 0;
+    HRF_CHECK_ARG(x && q && scale, "NULL argument");
+    HRF_CHECK_ARG((ldx >= cols || rows == 1) && ldq >= cols && ldq <= HRF_INT8_MAX_INNER + 1, "a row stride is shorter than the row, or that of q too long");
+    i8_rows<false>(x, x_type, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
     HRF_CHECK_LAUNCH();
     return 0;
 }
 
-template <int X>
-static void i8_float(const I8Args& A, const void* x, int64_t ldx, int64_t inner, int y_type, hipStream_t stream)
+extern "C" int hrf_int8_pack(const int8_t* q, int64_t rows, int64_t cols, int64_t ldq, int8_t* packed, hrf_stream_t stream)
 {
-    constexpr int size = (int)sizeof(typename I8Type<X>::T);
-    if (y_type == I8_F32) i8_short<X, I8_F32>(A, x, ldx, inner, size, stream);
-    else if (y_type == I8_F16) i8_short<X, I8_F16>(A, x, ldx, inner, size, stream);
-    else i8_short<X, I8_BF16>(A, x, ldx, inner, size, stream);
+    HRF_CHECK_ARG(rows >= 0 && rows < HRF_INT8_MAX_ROWS && i8_inner_ok(cols), "bad sizes");
+    if (rows == 0) return 0;
+    HRF_CHECK_ARG(q && packed, "NULL argument");
+    HRF_CHECK_ARG(ldq >= cols || rows == 1, "a row stride is shorter than the row");
+    HRF_CHECK_ARG(((uintptr_t)packed & 15u) == 0, "the packed codes must begin at a multiple of 16 bytes");
+    HRF_CHECK_ARG(hrf_int8_packed_bytes(rows, cols) < (int64_t)16 * 256 * 2147483647, "too many codes");
+    i8_pack(q, rows, cols, ldq, packed, (hipStream_t)stream);
+    HRF_CHECK_LAUNCH();
+    return 0;
 }
 
-extern "C" int64_t hrf_linear_int8_workspace_bytes(int64_t rows, int64_t cols, int64_t inner)
+extern "C" int hrf_linear_int8(const void* x, int x_type, int64_t ldx, const float* x_scale, const int8_t* w, const float* w_scale,
+                               const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
+                               void* workspace, hrf_stream_t stream)
 {
-    if (rows <= 0 || cols <= 0 || inner < 1 || inner > HRF_INT8_MAX_INNER) return 0;
-    return i8_is_short(rows, cols, i8_padded(inner)) ? 0 : rows * i8_padded(inner) + ((rows * 4 + 15) & ~(int64_t)15);
-}
-
-extern "C" int hrf_linear_int8_float(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
-                                     int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu, void* workspace,
-                                     hrf_stream_t stream)
-{
-    HRF_CHECK_ARG(x_type >= I8_F32 && x_type <= I8_BF16, "x_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
-    HRF_CHECK_ARG(inner >= 1 && inner <= HRF_INT8_MAX_INNER, "bad sizes");
-    const int64_t need = hrf_linear_int8_workspace_bytes(rows, cols, inner), padded = i8_padded(inner);
-    int rc = i8_check(__func__, (const void*)16, padded, (const float*)16, w, ldw, w_scale, rows, cols, padded, y, y_type, ldy);
-    if (rc || rows == 0 || cols == 0) return rc;
-    HRF_CHECK_ARG(x, "NULL argument");
-    HRF_CHECK_ARG(ldx >= inner || rows == 1, "a row stride is shorter than the row");
-    if (need > 0) {
-        HRF_CHECK_ARG(workspace && ((uintptr_t)workspace & 15u) == 0, "the workspace must begin at a multiple of 16 bytes");
-        float* const scale = (float*)((int8_t*)workspace + rows * padded);
-        rc = hrf_quantize_rows_int8(x, x_type, rows, inner, ldx, (int8_t*)workspace, padded, scale, stream);
-        return rc ? rc : hrf_linear_int8((const int8_t*)workspace, padded, scale, w, ldw, w_scale, bias, rows, cols, padded, y, y_type, ldy, relu, stream);
-    }
+    HRF_CHECK_ARG(x_type >= I8_F32 && x_type <= I8_INT8, "x_type must be 0 (fp32), 1 (fp16), 2 (bf16) or 3 (int8)");
+    HRF_CHECK_ARG(y_type >= I8_F32 && y_type <= I8_BF16, "y_type must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    HRF_CHECK_ARG(rows >= 0 && rows < HRF_INT8_MAX_ROWS && cols >= 0 && cols <= 64 * 65535 && i8_inner_ok(inner), "bad sizes");
+    HRF_CHECK_ARG(((rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 31) && hrf_int8_packed_bytes(rows, inner) < ((int64_t)1 << 42), "too many tiles");
+    if (rows == 0 || cols == 0) return 0;
+    HRF_CHECK_ARG(x && w && w_scale && y && (x_scale || x_type != I8_INT8), "NULL argument");
+    HRF_CHECK_ARG((ldx >= inner || rows == 1) && (ldy >= cols || rows == 1), "a row stride is shorter than the row");
+    HRF_CHECK_ARG(((uintptr_t)w & 15u) == 0, "w must begin at a multiple of 16 bytes");
+    HRF_CHECK_ARG(hrf_linear_int8_workspace_bytes(rows, cols, inner) == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0),
+                  "the workspace must begin at a multiple of 16 bytes");
     I8Args A;
-    A.x = nullptr; A.w = w; A.sx = nullptr; A.sw = w_scale; A.bias = bias; A.y = y; A.ldx = 0; A.ldw = ldw; A.ldy = ldy;
-    A.rows = (int)rows; A.cols = (int)cols; A.inner = (int)padded; A.relu = relu;
-    if (x_type == I8_F32) i8_float<I8_F32>(A, x, ldx, inner, y_type, (hipStream_t)stream);
-    else if (x_type == I8_F16) i8_float<I8_F16>(A, x, ldx, inner, y_type, (hipStream_t)stream);
-    else i8_float<I8_BF16>(A, x, ldx, inner, y_type, (hipStream_t)stream);
+    A.x = nullptr; A.ldx = 0; A.w = w; A.sx = nullptr; A.sw = w_scale; A.bias = bias; A.y = y; A.ldy = ldy;
+    A.rows = (int)rows; A.cols = (int)cols; A.inner = i8_padded(inner); A.relu = relu;
+    if (y_type == I8_F32) i8_product<I8_F32>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    else if (y_type == I8_F16) i8_product<I8_F16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    else i8_product<I8_BF16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
     HRF_CHECK_LAUNCH();
     return 0;
 }

@@ -10,13 +10,13 @@ from . import ops
 
 
 class Int8Linear(torch.nn.Module):
-    """y = act(x W^T + b), W in 8 bits: buffers `codes` (out, padded in), `scale` (out), `bias` (out) or None."""
+    """y = act(x W^T + b), W in 8 bits: buffers `packed` (codes), `scale` (out), `bias` (out) or None."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor = None, relu: bool = False):
         super().__init__()
         handle = ops.Int8Weight.from_float(weight, bias)
         self.in_features, self.out_features, self.relu = handle.in_features, handle.out_features, bool(relu)
-        self.register_buffer("codes", handle.codes)
+        self.register_buffer("packed", handle.packed)
         self.register_buffer("scale", handle.scale)
         self.register_buffer("bias", handle.bias)
         self._handle = handle
@@ -39,7 +39,7 @@ class Int8Linear(torch.nn.Module):
     @torch.no_grad()
     def forward(self, x: torch.Tensor, out_dtype=None) -> torch.Tensor:
         if self._handle is None:
-            self._handle = ops.Int8Weight.from_padded(self.codes, self.in_features, self.scale, self.bias)
+            self._handle = ops.Int8Weight.from_packed(self.packed, self.out_features, self.in_features, self.scale, self.bias)
         return ops.linear_int8(x.detach(), self._handle, relu=self.relu, out_dtype=out_dtype)
 
     def extra_repr(self) -> str:

@@ -840,35 +840,30 @@ def quantize_int8(x: torch.Tensor):
     return (q[:, :k] if x.dim() == 2 else q.view(*x.shape[:-1], q.shape[1])[..., :k]), scale.view(x.shape[:-1])
 
 
-def _padded_int8(rows: torch.Tensor) -> torch.Tensor:
-    """int8 rows as the product reads them: (rows, int8_padded(cols)), zeros behind the true length, 16-byte aligned; a copy unless
-    the rows lie like that already."""
-    m, k = rows.shape
-    if k == int8_padded(k) and rows.data_ptr() % 16 == 0 and (m == 1 or (rows.stride(0) % 16 == 0 and rows.stride(0) < 1 << 23)):
-        return rows
-    q = torch.empty(m, int8_padded(k), dtype=torch.int8, device=rows.device)
-    with _on_device(rows.device):
-        check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), 3, m, k, rows.stride(0), ptr(q), q.shape[1], None, stream_ptr()))
-    return q
-
-
 class Int8Weight:
-    """A layer's weights for linear_int8, laid out once: codes int8 (channels, inner), one fp32 scale per channel, fp32 bias per channel
-    or None. Codes whose rows are whole multiples of the padded length are kept as they are (not copied); write new values through a new
-    handle. `from_float` rounds a weight matrix (channels, inner)."""
+    """A layer's weights for linear_int8, laid out once: from codes int8 (channels, inner), one fp32 scale per channel and an fp32 bias per
+    channel or None. `packed` holds a copy of the codes in the order in which the product reads them (hrf_int8_pack, include/hrf.h); scale
+    and bias are kept, not copied. `from_float` rounds a weight matrix (channels, inner)."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
         if codes.dim() != 2 or codes.dtype != torch.int8:
             raise RuntimeError("Int8Weight: codes must be an int8 matrix (channels, inner)")
         rows = _rows_of(codes, "codes")
-        self.out_features, self.in_features, self.device = codes.shape[0], codes.shape[1], codes.device
+        n, k = rows.shape
+        packed = torch.empty(-(-n // 16), int8_padded(k) // 64, 64, 16, dtype=torch.int8, device=codes.device)
+        with _on_device(codes.device):
+            check(_lib.lib().hrf_int8_pack(ptr(rows), n, k, rows.stride(0), ptr(packed), stream_ptr()))
+        self._take(packed, n, k, scale, bias)
+
+    def _take(self, packed, out_features, in_features, scale, bias) -> None:
+        self.packed, self.out_features, self.in_features, self.device = packed, out_features, in_features, packed.device
         for t, name in ((scale, "scale"), (bias, "bias")):
             if t is None:
                 continue
             _chk(t, name, torch.float32)
-            if t.shape != (self.out_features,) or t.device != codes.device:
+            if t.shape != (out_features,) or t.device != packed.device:
                 raise RuntimeError(f"Int8Weight: {name} must hold one value per channel on the codes' device")
-        self.codes, self.scale, self.bias = _padded_int8(rows), scale, bias
+        self.scale, self.bias = scale, bias
 
     @classmethod
     def from_float(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Weight":
@@ -878,12 +873,14 @@ class Int8Weight:
         return cls(codes, scale, None if bias is None else bias.detach().float().contiguous())
 
     @classmethod
-    def from_padded(cls, codes: torch.Tensor, in_features: int, scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Weight":
-        """`codes` (channels, int8_padded(in_features)) of another handle, zeros behind in_features: kept, not copied."""
-        if codes.dim() != 2 or codes.shape[1] != int8_padded(int(in_features)):
-            raise RuntimeError(f"Int8Weight: padded codes have {int8_padded(int(in_features))} values a row")
-        self = cls(codes, scale, bias)
-        self.in_features = int(in_features)
+    def from_packed(cls, packed: torch.Tensor, out_features: int, in_features: int, scale: torch.Tensor,
+                    bias: Optional[torch.Tensor] = None) -> "Int8Weight":
+        """`packed` of another handle over weights of the same shape: kept, not copied."""
+        _chk(packed, "packed codes", torch.int8)
+        if packed.shape != (-(-int(out_features) // 16), int8_padded(int(in_features)) // 64, 64, 16) or packed.data_ptr() % 16:
+            raise RuntimeError("Int8Weight: the packed codes are of another shape, or do not begin at a multiple of 16 bytes")
+        self = cls.__new__(cls)
+        self._take(packed, int(out_features), int(in_features), scale, bias)
         return self
 
 
@@ -914,19 +911,12 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, x_scale: Optional[torch.Ten
     y = torch.empty(*x.shape[:-1], weight.out_features, dtype=out_dtype, device=x.device)
     if y.numel() == 0:
         return y
-    w, lib = weight.codes, _lib.lib()
+    n, lib = weight.out_features, _lib.lib()
     with _on_device(x.device), _span("linear_int8", m):
-        if x_scale is None:
-            need = lib.hrf_linear_int8_workspace_bytes(m, weight.out_features, k)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            check(lib.hrf_linear_int8_float(ptr(rows), _INT8_KINDS[x.dtype], rows.stride(0), ptr(w), w.stride(0), ptr(weight.scale),
-                                            ptr(weight.bias), m, weight.out_features, k, ptr(y), _INT8_KINDS[out_dtype],
-                                            weight.out_features, 1 if relu else 0, ptr(ws), stream_ptr()))
-        else:
-            codes = _padded_int8(rows)
-            check(lib.hrf_linear_int8(ptr(codes), codes.stride(0), ptr(x_scale), ptr(w), w.stride(0), ptr(weight.scale), ptr(weight.bias),
-                                      m, weight.out_features, w.shape[1], ptr(y), _INT8_KINDS[out_dtype], weight.out_features,
-                                      1 if relu else 0, stream_ptr()))
+        need = lib.hrf_linear_int8_workspace_bytes(m, n, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        check(lib.hrf_linear_int8(ptr(rows), _INT8_KINDS[x.dtype], rows.stride(0), ptr(x_scale), ptr(weight.packed), ptr(weight.scale),
+                                  ptr(weight.bias), m, n, k, ptr(y), _INT8_KINDS[out_dtype], n, 1 if relu else 0, ptr(ws), stream_ptr()))
     return y
 
 

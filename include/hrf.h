@@ -566,25 +566,26 @@ int hrf_grad_norm_multi(const hrf_adamw_tensor* tensors, const int32_t* tile_ten
 /* ------------------------------------------------------------------ 8-bit integer product -- */
 /* y[m][n] = act((sum_k x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]): a layer served with 8-bit weights, a scale for each
  * channel n and each token m; integer sums are exact. No counterpart in the reference, whose networks are fp16 (humanrf.py:123-156).
- * x (rows, inner), w (cols, inner) int8, row strides ldx, ldw: both begin at multiples of 16 bytes, `inner` is a padded length
- * (hrf_int8_padded: 64, or a multiple of 128; HRF_INT8_MAX_INNER before padding keeps the sums inside int32) and the bytes from the true length to `inner`
- * are zero. bias (cols) fp32 or NULL; relu != 0: max(., 0). y: row stride ldy (in values), y_type 0 fp32, 1 fp16, 2 bf16. */
+ * x: rows of `inner` values (1 .. HRF_INT8_MAX_INNER, which keeps the sums inside int32), row stride ldx in values, any alignment; x_type
+ * 0 fp32, 1 fp16, 2 bf16: each row is rounded to 8 bits with a scale of its own, as hrf_quantize_rows_int8 does; 3: int8 codes with x_scale (rows).
+ * w: codes of the (cols, inner) weights, packed by hrf_int8_pack. bias (cols) fp32 or NULL; relu != 0: max(., 0). y: row stride ldy (in
+ * values), y_type 0 fp32, 1 fp16, 2 bf16. cols <= 64 * 65535.
+ * workspace: DEVICE scratch of hrf_linear_int8_workspace_bytes() bytes (may be 0, then NULL), at a multiple of 16 bytes; no contents are kept. */
 #define HRF_INT8_MAX_INNER 131071
-#define HRF_INT8_MAX_STRIDE (1 << 23) /* row strides of x and w are smaller; cols is at most 64 * 65535 */
-int64_t hrf_int8_padded(int64_t cols);
-int hrf_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale,
-                    const float* bias, int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu,
-                    hrf_stream_t stream);
-/* The same with x in fp32, fp16 or bf16 (x_type 0, 1, 2; row stride ldx in values, `inner` its true length, any alignment): each row is
- * rounded to 8 bits with a scale of its own, as hrf_quantize_rows_int8 does, then multiplied. w as above, its rows padded to
- * hrf_int8_padded(inner). workspace: DEVICE scratch of hrf_linear_int8_workspace_bytes() bytes (may be 0), a multiple of 16 bytes. */
+#define HRF_INT8_MAX_ROWS 2147483392
 int64_t hrf_linear_int8_workspace_bytes(int64_t rows, int64_t cols, int64_t inner);
-int hrf_linear_int8_float(const void* x, int x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
-                          int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu, void* workspace,
-                          hrf_stream_t stream);
+int hrf_linear_int8(const void* x, int x_type, int64_t ldx, const float* x_scale, const int8_t* w, const float* w_scale, const float* bias,
+                    int64_t rows, int64_t cols, int64_t inner, void* y, int y_type, int64_t ldy, int relu, void* workspace,
+                    hrf_stream_t stream);
+/* Codes (rows, cols) int8, row stride ldq -> packed, hrf_int8_packed_bytes(rows, cols) bytes at a multiple of 16: rows padded with zeros to
+ * hrf_int8_padded(cols) (64, or the next multiple of 128), rows to a multiple of 16; blocks of 16 rows x 64 bytes, block (i, j) at
+ * (i * padded / 64 + j) * 1024, bytes 16 q .. 16 q + 15 of its row t at 256 q + 16 t. */
+int64_t hrf_int8_padded(int64_t cols);
+int64_t hrf_int8_packed_bytes(int64_t rows, int64_t cols);
+int hrf_int8_pack(const int8_t* q, int64_t rows, int64_t cols, int64_t ldq, int8_t* packed, hrf_stream_t stream);
 /* Rows of x (x_type 0 fp32, 1 fp16, 2 bf16; row stride ldx) -> codes q (row stride ldq >= cols, filled with zeros behind cols) and one
  * scale a row: scale = a * (1 / 127), q = rint(x * (127 / a)), a = max(max |x|, 2^-119). A row that is not finite gets codes 0 and a
- * scale that is not finite. x_type 3: int8 rows are copied, with the padding (scale is not written and may be NULL). */
+ * scale that is not finite. */
 int hrf_quantize_rows_int8(const void* x, int x_type, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                            hrf_stream_t stream);
 

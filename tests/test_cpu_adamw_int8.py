@@ -92,18 +92,19 @@ def test_the_optimizer_refuses():
 
 # ------------------------------------------------------------------------------------------------ 8-bit integer product
 def _linear(lib, **change):
-    a = dict(x=FAKE, ldx=128, x_scale=FAKE, w=FAKE, ldw=128, w_scale=FAKE, bias=None, rows=4, cols=8, inner=128, y=FAKE, y_type=0, ldy=8,
-             relu=0, stream=None)
+    a = dict(x=FAKE, x_type=2, ldx=100, x_scale=None, w=FAKE, w_scale=FAKE, bias=None, rows=4, cols=8, inner=100, y=FAKE, y_type=0, ldy=8, relu=0,
+             workspace=FAKE, stream=None)
     a.update(change)
     return lib.hrf_linear_int8(*a.values())
 
 
 @pytest.mark.parametrize("change,said", [
-    (dict(y_type=3), b"y_type"), (dict(y_type=-1), b"y_type"), (dict(rows=-1), b"sizes"), (dict(cols=-1), b"sizes"),
-    (dict(rows=2 ** 31), b"sizes"), (dict(inner=0), b"inner"), (dict(inner=100), b"inner"), (dict(inner=192), b"inner"),
-    (dict(inner=131200, ldx=131200, ldw=131200), b"inner"), (dict(x=None), b"NULL"), (dict(w=None), b"NULL"), (dict(y=None), b"NULL"),
-    (dict(x_scale=None), b"NULL"), (dict(w_scale=None), b"NULL"), (dict(ldx=64), b"stride"), (dict(ldw=112), b"stride"),
-    (dict(ldy=7), b"stride"), (dict(ldx=136), b"multiples of 16"), (dict(x=FAKE + 8), b"multiples of 16"), (dict(w=FAKE + 1), b"multiples of 16"),
+    (dict(x_type=4), b"x_type"), (dict(x_type=-1), b"x_type"), (dict(y_type=3), b"y_type"), (dict(y_type=-1), b"y_type"),
+    (dict(rows=-1), b"sizes"), (dict(cols=-1), b"sizes"), (dict(rows=2 ** 31), b"sizes"), (dict(cols=64 * 65535 + 1, ldy=1 << 40), b"sizes"),
+    (dict(inner=0), b"sizes"), (dict(inner=131072, ldx=131072), b"sizes"), (dict(rows=2 ** 31 - 300, cols=1 << 20, ldy=1 << 20), b"tiles"),
+    (dict(x=None), b"NULL"), (dict(w=None), b"NULL"), (dict(y=None), b"NULL"), (dict(w_scale=None), b"NULL"), (dict(x_type=3), b"NULL"),
+    (dict(ldx=99), b"stride"), (dict(ldy=7), b"stride"), (dict(w=FAKE + 8), b"multiple of 16"), (dict(workspace=None), b"workspace"),
+    (dict(workspace=FAKE + 8), b"workspace"),
 ])
 def test_the_product_refuses(change, said):
     from humanrf_amd import _lib
@@ -117,13 +118,14 @@ def test_products_of_nothing_are_nothing():
     lib = _lib.lib()
     assert _linear(lib, rows=0, x=None, y=None) == 0 and _linear(lib, cols=0, w=None, y=None) == 0
     assert lib.hrf_quantize_rows_int8(None, 0, 0, 5, 5, None, 64, None, None) == 0
+    assert lib.hrf_int8_pack(None, 0, 5, 5, None, None) == 0
 
 
 @pytest.mark.parametrize("args", [
-    (FAKE, 4, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, -1, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, 0, -1, 5, 5, FAKE, 64, FAKE, None),
+    (FAKE, 3, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, -1, 2, 5, 5, FAKE, 64, FAKE, None), (FAKE, 0, -1, 5, 5, FAKE, 64, FAKE, None),
     (FAKE, 0, 2, 0, 5, FAKE, 64, FAKE, None), (FAKE, 0, 2, 131072, 131072, FAKE, 131072, FAKE, None), (None, 0, 2, 5, 5, FAKE, 64, FAKE, None),
     (FAKE, 0, 2, 5, 5, None, 64, FAKE, None), (FAKE, 0, 2, 5, 5, FAKE, 64, None, None), (FAKE, 0, 2, 5, 4, FAKE, 64, FAKE, None),
-    (FAKE, 0, 2, 5, 5, FAKE, 4, FAKE, None),
+    (FAKE, 0, 2, 5, 5, FAKE, 4, FAKE, None), (FAKE, 0, 2, 5, 5, FAKE, 131073, FAKE, None),
 ])
 def test_rounding_rows_refuses(args):
     from humanrf_amd import _lib
@@ -132,20 +134,15 @@ def test_rounding_rows_refuses(args):
     assert b"hrf_quantize_rows_int8" in lib.hrf_last_error()
 
 
-@pytest.mark.parametrize("change,said", [
-    (dict(x_type=3), b"x_type"), (dict(inner=0), b"sizes"), (dict(inner=131072), b"sizes"), (dict(x=None), b"NULL"), (dict(w=None), b"NULL"),
-    (dict(ldx=99), b"stride"), (dict(ldw=96), b"stride"), (dict(y_type=9), b"y_type"), (dict(workspace=None), b"workspace"),
-    (dict(workspace=FAKE + 8), b"workspace"), (dict(rows=-5), b"sizes"),
+@pytest.mark.parametrize("args", [
+    (FAKE, -1, 5, 5, FAKE, None), (FAKE, 2, 0, 5, FAKE, None), (FAKE, 2, 131072, 131072, FAKE, None), (None, 2, 5, 5, FAKE, None),
+    (FAKE, 2, 5, 5, None, None), (FAKE, 2, 5, 4, FAKE, None), (FAKE, 2, 5, 5, FAKE + 4, None),
 ])
-def test_the_product_of_float_rows_refuses(change, said):
+def test_packing_refuses(args):
     from humanrf_amd import _lib
     lib = _lib.lib()
-    a = dict(x=FAKE, x_type=2, ldx=100, w=FAKE, ldw=128, w_scale=FAKE, bias=None, rows=4, cols=8, inner=100, y=FAKE, y_type=0, ldy=8, relu=0,
-             workspace=FAKE, stream=None)
-    a.update(change)
-    assert lib.hrf_linear_int8_float(*a.values()) != 0
-    assert b"hrf_linear_int8_float" in lib.hrf_last_error() and said in lib.hrf_last_error()
-    assert lib.hrf_linear_int8_workspace_bytes(-1, 8, 100) == 0 and lib.hrf_linear_int8_workspace_bytes(4, 8, 100) >= 4 * (128 + 4)
+    assert lib.hrf_int8_pack(*args) != 0
+    assert b"hrf_int8_pack" in lib.hrf_last_error()
 
 
 def test_padded_lengths():
@@ -154,6 +151,10 @@ def test_padded_lengths():
     assert [lib.hrf_int8_padded(k) for k in (0, 131072)] == [-1, -1]
     for k in (1, 63, 64, 65, 127, 128, 129, 2051, 131071):
         assert lib.hrf_int8_padded(k) == ops.int8_padded(k) >= k
+        assert lib.hrf_int8_packed_bytes(17, k) == 32 * ops.int8_padded(k)
+    assert lib.hrf_int8_packed_bytes(-1, 5) == -1 and lib.hrf_int8_packed_bytes(5, 0) == -1
+    assert lib.hrf_linear_int8_workspace_bytes(-1, 8, 100) == 0 and lib.hrf_linear_int8_workspace_bytes(4, 8, 100) == 16 * 128 + 16
+    assert lib.hrf_linear_int8_workspace_bytes(10_000, 64, 64) == 0
 
 
 def test_the_wrappers_refuse():

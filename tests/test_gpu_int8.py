@@ -167,24 +167,40 @@ def test_refusals_on_the_device():
         ops.linear_int8(torch.zeros(32, 4, device="cuda").t(), h)
     with pytest.raises(RuntimeError, match="one value per channel"):
         ops.Int8Weight(w, sx)
+    with pytest.raises(RuntimeError, match="another shape"):
+        ops.Int8Weight.from_packed(h.packed, 17, 32, torch.ones(17, device="cuda"))
     with pytest.raises(RuntimeError, match="1 to"):
         ops.quantize_int8(torch.zeros(2, 131072, device="cuda"))
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
         ops.quantize_int8(x)
 
 
+def test_packed_codes():
+    from humanrf_amd import ops
+    for n, k in ((1, 1), (16, 64), (17, 65), (40, 300)):
+        _, w, _, sw, _ = _case(1, n, k)
+        p = ops.Int8Weight(w, sw).packed
+        rows, cols = -(-n // 16) * 16, ops.int8_padded(k)
+        full = torch.zeros(rows, cols, dtype=torch.int8, device="cuda")
+        full[:n, :k] = w
+        # block (i, j), byte 256 q + 16 t + b: row 16 i + t, code 64 j + 16 q + b
+        assert torch.equal(p.view(rows // 16, cols // 64, 4, 16, 16), full.view(rows // 16, 16, cols // 64, 4, 16).permute(0, 2, 3, 1, 4))
+
+
 def test_what_lies_around_stays():
-    """y is written inside its rows and nowhere else; nothing past the ends of x and W is needed: both end their storage here."""
+    """y is written inside its rows and nowhere else; x ends its storage here."""
     from humanrf_amd import _lib, ops
     from humanrf_amd._lib import check, ptr, stream_ptr
-    for m, n, k in ((1, 70, 128), (20, 70, 128), (200, 130, 256), (700, 50, 64)):
+    for m, n, k in ((1, 70, 128), (20, 70, 128), (200, 130, 256), (700, 50, 64), (5000, 50, 100)):
         x, w, sx, sw, b = _case(m, n, k)
+        h = ops.Int8Weight(w, sw, b)
         y = torch.full((m + 2, n + 9), 55.0, dtype=F16, device="cuda")
-        check(_lib.lib().hrf_linear_int8(ptr(x), k, ptr(sx), ptr(w), k, ptr(sw), ptr(b), m, n, k, y[1].data_ptr(), 1, n + 9, 0, stream_ptr()))
+        ws = torch.empty(_lib.lib().hrf_linear_int8_workspace_bytes(m, n, k), dtype=torch.uint8, device="cuda")
+        check(_lib.lib().hrf_linear_int8(ptr(x), 3, k, ptr(sx), ptr(h.packed), ptr(sw), ptr(b), m, n, k, y[1].data_ptr(), 1, n + 9, 0, ptr(ws) or None,
+                                         stream_ptr()))
         _holds(y[1:1 + m, :n].contiguous(), x, w, sx, sw, b, False)
         y[1:1 + m, :n] = 55.0
         assert bool((y == 55.0).all())
-    assert ops.int8_padded(64) == 64
 
 
 def test_offsets_past_32_bits():
