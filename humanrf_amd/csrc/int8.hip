@@ -228,39 +228,42 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
     tn = in / height;
 }
 
-// Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 128
-// bytes of k in LDS, two stages, filled by direct loads (16 bytes a lane, no registers). W's packed blocks lie there as in memory: 16
-// lanes that read together read 256 bytes side by side. A token's eight 16-byte chunks lie permuted by its number, so that lanes that
-// read the same chunk of neighbouring tokens hit all banks.
-// The operands of the next 32 k are read from LDS while the matrix cores work on these; before the last 32 k of a stage the workgroup
-// meets, the loads of the stage after the next take the buffer that everybody has read, and the next stage's first operands follow.
-// LDS is what bounds smaller tiles: it gives 128 bytes a clock, and 128 x 128 tiles ask for 187 where 256 x 256 ask for 94. 8192^3:
-// 897 us with 128 x 128 tiles, 540 us (2.04 POP/s) with 256 x 256; the library's product of the same integers reaches 2.14.
+// Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 64
+// bytes of k in LDS, four stages, filled by direct loads (16 bytes a lane, no registers) three stages ahead. W's packed blocks lie there as
+// in memory: 16 lanes that read together read 256 bytes side by side. A token's four 16-byte chunks lie permuted by its number, so that 16
+// lanes that read the same chunk of neighbouring tokens hit all 64 banks.
+// Everything is dealt out between the products: while the matrix cores work on 32 k, the operands of the next 32 are read from LDS and
+// a quarter of the loads of the third stage on is issued (sixteen loads in a row hold the wavefront up for as long as they take
+// to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
+// LDS is what bounds smaller tiles. 8192^3: 897 us with 128 x 128 tiles, 483 us (2.27 POP/s) with 256 x 256; the library's product of
+// the same integers reaches 2.14.
 template <int K, int TM, int TN>
 __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const I8Args A)
 {
-    constexpr int BM = 64 * TM, BN = 64 * TN, kStage = (BM + BN) * 128, kLoads = (BM + BN) / 32;
+    constexpr int BM = 64 * TM, BN = 64 * TN, kStage = (BM + BN) * 64, kLoads = (BM + BN) / 64;      // loads of a wavefront a stage
+    constexpr int kGroups = kLoads / 2, kReads = (TM + TN) / kGroups, kProducts = TM * TN / kGroups;
     typedef typename I8Type<K>::T T;
     typedef int i8_v16 __attribute__((ext_vector_type(16)));
-    __shared__ __align__(16) int8_t s_tile[2 * kStage];
+    __shared__ __align__(16) int8_t s_tile[4 * kStage];
     __shared__ float s_sx[BM], s_sw[BN], s_bias[BN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
     int tm, tn;
     i8_tile_of((A.rows + BM - 1) / BM, (A.cols + BN - 1) / BN, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int steps = A.inner >> 7;
+    const int steps = A.inner >> 6;
 
-    // Load i of the wavefronts 0, 1: eight tokens, this lane's row first + lane / 8 (past the end: the last one), its chunk permuted.
-    // Of the wavefronts 2, 3: half a stage of 16 channels, a block (past the end: the last one).
+    // Load i of the wavefronts 0, 1: 16 tokens, this lane's row lane / 4 of them (past the end: the last one), its chunk permuted.
+    // Of the wavefronts 2, 3: a block of 16 channels (past the end: the last one).
     uint32_t from[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-        from[i] = wave < 2 ? (uint32_t)min((wave * kLoads + i) * 8 + (lane >> 3), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 7) ^ (lane >> 3)) * 16
-                           : (uint32_t)(min((n0 >> 4) + ((wave - 2) * kLoads + i) / 2, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + (i & 1) * 1024 + lane * 16;
+        from[i] = wave < 2 ? (uint32_t)min((wave * kLoads + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
+                           : (uint32_t)(min((n0 >> 4) + (wave - 2) * kLoads + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
     const int8_t* const base = wave < 2 ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
-    const int forward = wave < 2 ? 128 : 2048;
+    const int forward = wave < 2 ? 64 : 1024;
     const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kLoads * 1024;
-    auto load = [&](int i, int buf, int s) { i8_load_lds(base + (int64_t)s * forward, from[i], lds + buf * kStage + i * 1024); };
+    auto load = [&](int i, int s) { i8_load_lds(base + (int64_t)min(s, steps - 1) * forward, from[i], lds + (s & 3) * kStage + i * 1024); };
+
     i8_v16 acc[TN][TM];
 #pragma unroll
     for (int a = 0; a < TN; ++a)
@@ -268,22 +271,27 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
         for (int b = 0; b < TM; ++b)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[a][b][k] = 0;
-    i8_v4 fx[2][TM], fw[2][TN];
-    const int x_row = (wm * 32 * TM + (lane & 31)) * 128;
-    const int w_row = (BM / 16 + wn * 2 * TN) * 2048 + ((lane >> 4) & 1) * 2048 + (lane >> 5) * 256 + (lane & 15) * 16;
-    auto read = [&](int set, int buf, int kk) {
-        const int8_t* t = s_tile + buf * kStage;
-        const int chunk = ((kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16;
-#pragma unroll
-        for (int b = 0; b < TM; ++b) fx[set][b] = *(const i8_v4*)(t + x_row + chunk + b * 4096);
-#pragma unroll
-        for (int a = 0; a < TN; ++a) fw[set][a] = *(const i8_v4*)(t + w_row + kk * 512 + a * 4096);
+    i8_v4 fr[2][TM + TN];       // two sets of operands: of the tokens, then of the channels
+    const int x_row = (wm * 32 * TM + (lane & 31)) * 64, w_row = (BM / 16 + wn * 2 * TN) * 1024 + ((lane >> 4) & 1) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
+    auto read = [&](int set, int j, int s, int kk) {
+        const int8_t* t = s_tile + (s & 3) * kStage;
+        if (j < TM) fr[set][j] = *(const i8_v4*)(t + x_row + ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16 + j * 2048);
+        else fr[set][j] = *(const i8_v4*)(t + w_row + kk * 512 + (j - TM) * 2048);
     };
-    auto multiply = [&](int set) {
+    // the products of one set, between them the reads of the other (k half `kk` of stage `next`) and half of the loads of stage `ahead`
+    auto work = [&](int set, int next, int kk, int ahead) {
 #pragma unroll
-        for (int a = 0; a < TN; ++a)
+        for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-            for (int b = 0; b < TM; ++b) acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][a], fx[set][b], acc[a][b], 0, 0, 0);
+            for (int j = 0; j < kReads; ++j) read(set ^ 1, g * kReads + j, next, kk);
+#pragma unroll
+            for (int p = 0; p < kProducts; ++p) {
+                const int a = (g * kProducts + p) / TM, b = (g * kProducts + p) % TM;
+                acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][TM + a], fr[set][b], acc[a][b], 0, 0, 0);
+            }
+            load(set * kGroups + g, ahead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     for (int k = threadIdx.x; k < BM; k += 256) s_sx[k] = A.sx[min(m0 + k, A.rows - 1)];
     for (int k = threadIdx.x; k < BN; k += 256) {
@@ -292,38 +300,19 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
         s_bias[k] = A.bias ? A.bias[n] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load(i, 0, 0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (steps > 1) {
+    for (int s = 0; s < 3; ++s)
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(i, 1, 1);
+        for (int i = 0; i < kLoads; ++i) load(i, s);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
+#pragma unroll
+    for (int j = 0; j < TM + TN; ++j) read(0, j, 0, 0);
+    for (int s = 0; s < steps; ++s) {
+        work(0, s, 1, s + 3);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + kGroups) : "memory");   // stage s + 1 has landed, of two more 3 halves are on their way
+        work(1, s + 1, 0, s + 3);       // (past the end: stages that are there, read again and not used)
     }
-    read(0, 0, 0);
-    auto three = [&](int buf) {
-#pragma unroll
-        for (int kk = 0; kk < 3; ++kk) {
-            read((kk + 1) & 1, buf, kk + 1);
-            multiply(kk & 1);
-#pragma unroll
-            for (int i = 0; i < TM + TN; ++i) {     // one operand read for every TM TN / (TM + TN) products
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, TM * TN / (TM + TN), 0);
-            }
-        }
-    };
-    for (int s = 0; s + 1 < steps; ++s) {
-        const int buf = s & 1;
-        three(buf);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");     // the next stage has landed, this one is in registers
-        read(0, buf ^ 1, 0);
-        if (s + 2 < steps) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) load(i, buf, s + 2);
-        }
-        multiply(1);
-    }
-    three((steps - 1) & 1);
-    multiply(1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // nothing may land in LDS that is somebody else's by then
+
     // Epilogue, 32 channels of 32 tokens at a time: a lane holds channels 8 g + 4 (lane / 32) + 0 .. 3 of token lane % 32. For 16-bit y the
     // halves of the wavefront trade, so that a lane has eight neighbouring channels, 16 bytes. (Through LDS, whole rows at a time, this
     // took as long as 2000 k of products: there is no other workgroup on the CU to work meanwhile.)
