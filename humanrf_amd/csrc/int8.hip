@@ -527,6 +527,91 @@ __global__ __launch_bounds__(64 * kWaves) void k_linear_i8_few(const I8Args A)
     }
 }
 
+// The same for very few rows of floats, rounded by every workgroup for itself into LDS, so that there is one launch and nothing to wait for:
+// W's first operands are on their way meanwhile. Rows are dealt to groups of wavefronts; x is read twice, the second time from the
+// cache. See i8_is_one for when.
+template <int X, int K, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void k_linear_i8_one(const I8Args A, const I8Short B, int per_row)
+{
+    typedef typename I8Type<K>::T T;
+    typedef typename I8Type<X>::T XT;
+    constexpr int n = I8Piece<X>::n, kAhead = 8;
+    __shared__ i8_v4 s_part[kWaves][64];
+    __shared__ uint32_t s_top[kWaves];
+    __shared__ float s_scale[kWaves];
+    extern __shared__ __align__(16) int8_t s_x[];       // rows of inner + 16 codes
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = lane & 15, q = lane >> 4;
+    const int n0 = (int)blockIdx.x * 16;
+    const int runs = A.inner >> 6, each = (runs + kWaves - 1) / kWaves, begin = wave * each, end = min(begin + each, runs);
+    const int8_t* const w = A.w + (int64_t)blockIdx.x * runs * 1024 + lane * 16;
+    i8_v4 fw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) fw[u] = *(const i8_v4*)(w + (int64_t)max(min(begin + u, end - 1), 0) * 1024);
+
+    const int row = wave / per_row, part = wave % per_row, stride = A.inner + 16;
+    const bool mine = row < A.rows;
+    const XT* const from = (const XT*)B.x + (int64_t)(mine ? row : 0) * B.ldx;
+    auto get = [&](int k0, I8Piece<X>& v) {
+        if (k0 + n <= B.inner) i8_get<X>(v, from + k0);
+        else {
+#pragma unroll
+            for (int k = 0; k < n; ++k) v.v[k] = k0 + k < B.inner ? from[k0 + k] : I8Type<X>::down(0.0f);
+        }
+    };
+    uint32_t top = 0;
+    if (mine)
+        for (int k0 = (part * 64 + lane) * n; k0 < B.inner; k0 += per_row * 64 * n) {
+            I8Piece<X> v;
+            get(k0, v);
+#pragma unroll
+            for (int k = 0; k < n; ++k) top = max(top, i8_bits(I8Type<X>::up(v.v[k])));
+        }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    for (int p = 0; p < per_row; ++p) top = max(top, s_top[row * per_row + p]);
+    float sc;
+    const float factor = i8_factor(top, sc);
+    const bool finite = top < 0x7f800000u;
+    if (part == 0 && lane == 0) s_scale[row] = sc;
+    if (mine)
+        for (int k0 = (part * 64 + lane) * n; k0 < A.inner; k0 += per_row * 64 * n) {
+            I8Piece<X> v;
+            get(k0, v);
+            uint32_t word[n / 4];
+#pragma unroll
+            for (int i = 0; i < n / 4; ++i) {
+                word[i] = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) word[i] |= i8_code(I8Type<X>::up(v.v[4 * i + k]), factor, finite) << (8 * k);
+            }
+#pragma unroll
+            for (int i = 0; i < n / 4; ++i) *(uint32_t*)(s_x + row * stride + k0 + 4 * i) = word[i];
+        }
+    __syncthreads();
+    const int8_t* const x = s_x + min(t, A.rows - 1) * stride + q * 16;
+    i8_v4 acc = {0, 0, 0, 0};
+    for (int r = begin; r < end; r += kAhead) {
+        if (r > begin) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) fw[u] = *(const i8_v4*)(w + (int64_t)min(r + u, end - 1) * 1024);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (r + u < end) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], *(const i8_v4*)(x + (r + u) * 64), acc, 0, 0, 0);
+    }
+    s_part[wave][lane] = acc;
+    __syncthreads();
+    if (threadIdx.x >= 256) return;
+    const int nl = threadIdx.x & 15, m = threadIdx.x >> 4;
+    if (m >= A.rows || n0 + nl >= A.cols) return;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) sum += s_part[v][(nl >> 2) * 16 + m][nl & 3];
+    ((T*)A.y)[(int64_t)m * A.ldy + n0 + nl] = i8_finish<K>(sum, s_scale[m], A.sw[n0 + nl], A.bias ? A.bias[n0 + nl] : 0.0f, A.bias != nullptr, A.relu != 0);
+}
+
 static int i8_padded(int64_t cols) { return (int)(cols <= 64 ? 64 : (cols + 127) / 128 * 128); }
 
 // ldq: row stride of the codes, or their padded length when they are packed
@@ -577,6 +662,22 @@ static void i8_short(const I8Args& A, const I8Short& B, hipStream_t stream)
     else hipLaunchKernelGGL((k_linear_i8_short<X, K, 4>), grid, dim3(256), 0, stream, A, B);
 }
 
+// Very few rows, by the time of the captured call against rounding in a launch before: 1 x 4096 x 4096 6.6 us against 8.4, 1 x 4096 x 14336
+// 16.5 against 19.4, 2 x 4096 x 4096 7.5 against 8.4, 8 x 1024 x 1024 4.5 against 5.6; but 4 x 4096 x 4096 8.8 against 8.3 and
+// 4 x 28672 x 4096 36 against 27, each workgroup's share of the rounding growing with the rows.
+static bool i8_is_one(int64_t rows, int64_t padded, int x_type)
+{
+    return x_type != I8_INT8 && rows <= 8 && rows * padded <= (rows == 1 ? 32768 : 8192);
+}
+
+template <int X, int K>
+static void i8_one(const I8Args& A, const I8Short& B, hipStream_t stream)
+{
+    const dim3 grid((unsigned)((A.cols + 15) / 16));
+    const int groups = A.rows <= 1 ? 1 : A.rows <= 2 ? 2 : A.rows <= 4 ? 4 : 8;
+    hipLaunchKernelGGL((k_linear_i8_one<X, K, 8>), grid, dim3(512), (size_t)A.rows * (A.inner + 16), stream, A, B, 8 / groups);
+}
+
 template <int K, int MT, int NT>
 static void i8_few(const I8Args& A, hipStream_t stream)
 {
@@ -611,6 +712,14 @@ static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const 
         else if (x_type == I8_F16) i8_short<I8_F16, K>(A, B, stream);
         else if (x_type == I8_BF16) i8_short<I8_BF16, K>(A, B, stream);
         else i8_short<I8_INT8, K>(A, B, stream);
+        return;
+    }
+    if (i8_is_one(A.rows, A.inner, x_type)) {
+        I8Short B;
+        B.x = x; B.ldx = ldx; B.sx = nullptr; B.inner = inner;
+        if (x_type == I8_F32) i8_one<I8_F32, K>(A, B, stream);
+        else if (x_type == I8_F16) i8_one<I8_F16, K>(A, B, stream);
+        else i8_one<I8_BF16, K>(A, B, stream);
         return;
     }
     float* const scale = (float*)((int8_t*)workspace + ((int64_t)A.rows + 15) / 16 * 16 * A.inner);

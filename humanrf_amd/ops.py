@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, ptr, stream_of, stream_ptr
 
 STEP = 4e-4  # render_step_size / raymarching_step_size (data_loader.py:573, volume_rendering.py:47,92)
 
@@ -605,20 +605,9 @@ def adam_multi(descriptors: torch.Tensor, count: int, num_groups: int, max_eleme
                                         grad_scale, ptr(state), ptr(scaler), ptr(workspace), stream_ptr()))
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NOGUARD = _NoGuard()
-
-
 def _on_device(device: torch.device):
     """Context in which `device` is the current one (a launch goes to the current device, on ITS current stream)."""
-    return _NOGUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NOSPAN if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 _ADAMW_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -694,6 +683,11 @@ class AdamWPlan:
         self._desc = None
         self.grads = None
         self.set_grads([None] * len(params) if grads is None else grads)
+        # what the entry points take of the plan, as addresses: none of these buffers is ever replaced
+        st = list(self.state.values())
+        first, second, scales = (st[0], st[1], (None, None)) if self.state_bits == 32 else (st[0], st[2], (st[1], st[3]))
+        self._head = (ptr(self._desc), ptr(self._tile_tensor), self.num_tiles)
+        self._body = (len(params), self.state_bits, ptr(first), ptr(second), ptr(scales[0]), ptr(scales[1]), ptr(self._ctl))
 
     def _take_state(self, state):
         blocks = self.numel // self.BLOCK
@@ -764,8 +758,7 @@ def grad_norm_multi(plan: AdamWPlan, grad_scale: float = 1.0, scaler=None, out=N
     if scaler is not None and scaler.device != plan.device:
         raise RuntimeError("grad_norm_multi: the grad scaler lies on another device")
     with _on_device(plan.device), _span("grad_norm", plan.numel):
-        check(_lib.lib().hrf_grad_norm_multi(ptr(plan._desc), ptr(plan._tile_tensor), plan.num_tiles, float(grad_scale), ptr(scaler),
-                                             ptr(plan._ws), ptr(out), stream_ptr()))
+        check(_lib.lib().hrf_grad_norm_multi(*plan._head, float(grad_scale), ptr(scaler), ptr(plan._ws), ptr(out), stream_of(plan.device.index)))
     return out
 
 
@@ -789,15 +782,10 @@ def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weig
             raise RuntimeError("adamw_multi: lr, norm, flags and scaler hold a value")
     if max_norm is not None and (norm is None or not float(max_norm) > 0.0):
         raise RuntimeError("adamw_multi: max_norm is a positive number and needs the norm of the gradients")
-    st = list(plan.state.values())
-    if plan.state_bits == 32:
-        st = [st[0], None, st[1], None]
     with _on_device(plan.device), _span("adamw", plan.numel):
-        check(_lib.lib().hrf_adamw_multi(ptr(plan._desc), ptr(plan._tile_tensor), plan.num_tiles, len(plan.params), plan.state_bits,
-                                         ptr(st[0]), ptr(st[2]), ptr(st[1]), ptr(st[3]), ptr(plan._ctl), float(lr), ptr(lr_dev),
-                                         float(betas[0]), float(betas[1]), float(eps), float(weight_decay), float(grad_scale),
-                                         0.0 if max_norm is None else float(max_norm), ptr(norm), ptr(flags), ptr(scaler), plan.seed,
-                                         1 if zero_grad else 0, stream_ptr()))
+        check(_lib.lib().hrf_adamw_multi(*plan._head, *plan._body, float(lr), ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
+                                         float(weight_decay), float(grad_scale), 0.0 if max_norm is None else float(max_norm), ptr(norm),
+                                         ptr(flags), ptr(scaler), plan.seed, 1 if zero_grad else 0, stream_of(plan.device.index)))
 
 
 _INT8_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
@@ -836,7 +824,7 @@ def quantize_int8(x: torch.Tensor):
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
     with _on_device(x.device), _span("quantize_int8", m):
         check(_lib.lib().hrf_quantize_rows_int8(ptr(rows), _INT8_KINDS[x.dtype], m, k, rows.stride(0), ptr(q), q.shape[1], ptr(scale),
-                                                stream_ptr()))
+                                                stream_of(x.device.index)))
     return (q[:, :k] if x.dim() == 2 else q.view(*x.shape[:-1], q.shape[1])[..., :k]), scale.view(x.shape[:-1])
 
 
@@ -852,7 +840,7 @@ class Int8Weight:
         n, k = rows.shape
         packed = torch.empty(-(-n // 16), int8_padded(k) // 64, 64, 16, dtype=torch.int8, device=codes.device)
         with _on_device(codes.device):
-            check(_lib.lib().hrf_int8_pack(ptr(rows), n, k, rows.stride(0), ptr(packed), stream_ptr()))
+            check(_lib.lib().hrf_int8_pack(ptr(rows), n, k, rows.stride(0), ptr(packed), stream_of(codes.device.index)))
         self._take(packed, n, k, scale, bias)
 
     def _take(self, packed, out_features, in_features, scale, bias) -> None:
@@ -916,7 +904,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, x_scale: Optional[torch.Ten
         need = lib.hrf_linear_int8_workspace_bytes(m, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         check(lib.hrf_linear_int8(ptr(rows), _INT8_KINDS[x.dtype], rows.stride(0), ptr(x_scale), ptr(weight.packed), ptr(weight.scale),
-                                  ptr(weight.bias), m, n, k, ptr(y), _INT8_KINDS[out_dtype], n, 1 if relu else 0, ptr(ws), stream_ptr()))
+                                  ptr(weight.bias), m, n, k, ptr(y), _INT8_KINDS[out_dtype], n, 1 if relu else 0, ptr(ws), stream_of(x.device.index)))
     return y
 
 
