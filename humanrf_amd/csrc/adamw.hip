@@ -12,8 +12,9 @@
 // parameter with a first moment never divides by eps alone.
 //
 // Both passes stream: 28 B a parameter with fp32 p, g, m, v, 16.06 B with 8-bit states. On MI355X, where a copy of 4 GiB reads and writes
-// 5.0 TB/s: 39 M fp32 parameters and their fp16 copy 191 us (6.1 TB/s) with 32-bit states, bound by HBM, and 134 us (5.3 TB/s) with 8-bit
-// ones, where the vector unit (about 100 instructions an element) is busy for as long; the norm of 240 M fp32 gradients 161 us (6.0 TB/s).
+// 5.0 TB/s: 39 M fp32 parameters and their fp16 copy 191 us (6.1 TB/s) with 32-bit states, bound by HBM, and 131 us (5.4 TB/s) with 8-bit
+// ones, whose 88 vector instructions an element keep the vector unit busy three quarters of that time; the norm of 240 M fp32 gradients
+// 161 us (6.0 TB/s).
 #include "hrf_common.h"
 #include <cmath>
 
@@ -23,7 +24,11 @@
 
 typedef float aw_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t aw_u2 __attribute__((ext_vector_type(2)));
+// the same at any address of its values (unaligned accesses are the hardware's)
+typedef float aw_f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t aw_u2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t aw_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t aw_u4u __attribute__((ext_vector_type(4), aligned(2)));
 
 enum { AW_F32 = 0, AW_F16 = 1, AW_BF16 = 2 };
 
@@ -54,15 +59,14 @@ __device__ __forceinline__ uint32_t aw_narrow16(float x, bool bf16)   // round t
 // global_store and not flat accesses.
 #define AW_GLOBAL __attribute__((address_space(1)))
 
-// Four consecutive values of a tensor of type K. kFull: all four are there and the address is a multiple of the access; otherwise those
-// below n, one by one.
+// Four consecutive values of a tensor of type K. kFull: all four are there; otherwise those below n, one by one.
 template <int K, bool kFull>
 __device__ __forceinline__ void aw_load4(const void* base, int64_t i, int64_t n, float out[4])
 {
     if (K == AW_F32) {
         const AW_GLOBAL float* p = (const AW_GLOBAL float*)base + i;
         if (kFull) {
-            const aw_f4 x = __builtin_nontemporal_load((const AW_GLOBAL aw_f4*)p);
+            const aw_f4 x = __builtin_nontemporal_load((const AW_GLOBAL aw_f4u*)p);
 #pragma unroll
             for (int k = 0; k < 4; ++k) out[k] = x[k];
         } else {
@@ -72,7 +76,7 @@ __device__ __forceinline__ void aw_load4(const void* base, int64_t i, int64_t n,
     } else {
         const AW_GLOBAL uint16_t* p = (const AW_GLOBAL uint16_t*)base + i;
         if (kFull) {
-            const aw_u2 x = __builtin_nontemporal_load((const AW_GLOBAL aw_u2*)p);
+            const aw_u2 x = __builtin_nontemporal_load((const AW_GLOBAL aw_u2u*)p);
 #pragma unroll
             for (int k = 0; k < 4; ++k) out[k] = aw_widen16((x[k >> 1] >> (16 * (k & 1))) & 0xffffu, K == AW_BF16);
         } else {
@@ -87,7 +91,7 @@ __device__ __forceinline__ void aw_store4(void* base, int64_t i, int64_t n, cons
 {
     if (K == AW_F32) {
         AW_GLOBAL float* p = (AW_GLOBAL float*)base + i;
-        if (kFull) __builtin_nontemporal_store(aw_f4{in[0], in[1], in[2], in[3]}, (AW_GLOBAL aw_f4*)p);
+        if (kFull) __builtin_nontemporal_store(aw_f4{in[0], in[1], in[2], in[3]}, (AW_GLOBAL aw_f4u*)p);
         else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) if (i + k < n) p[k] = in[k];
@@ -99,8 +103,8 @@ __device__ __forceinline__ void aw_store4(void* base, int64_t i, int64_t n, cons
         for (int k = 0; k < 4; ++k) h[k] = aw_narrow16(in[k], K == AW_BF16);
         if (kFull) {
             const aw_u2 x = {h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
-            if (kKeep) *(AW_GLOBAL aw_u2*)p = x;     // (the 16-bit copy is what the next forward pass reads: it stays cacheable)
-            else __builtin_nontemporal_store(x, (AW_GLOBAL aw_u2*)p);
+            if (kKeep) *(AW_GLOBAL aw_u2u*)p = x;     // (the 16-bit copy is what the next forward pass reads: it stays cacheable)
+            else __builtin_nontemporal_store(x, (AW_GLOBAL aw_u2u*)p);
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) if (i + k < n) p[k] = (uint16_t)h[k];
@@ -168,11 +172,11 @@ __device__ __forceinline__ void aw_scale(uint32_t amax_bits, float& scale, float
 
 __device__ __forceinline__ float aw_round_e4m3(float ax, float inverse, uint32_t random16, bool floor)
 {
-    const float t = fminf(ax * inverse, 448.0f);
+    const float t = ax * inverse;       // (up to a rounding over 448)
     // below 2^-6 e4m3 values are 2^-9 apart, which is the gap of the binade [2^-6, 2^-5): move the value there and back
     const float low = t < 0x1p-6f ? 0x1p-6f : 0.0f;
     const uint32_t bits = (__float_as_uint(t + low) + (random16 << 4)) & 0xfff00000u;   // 3 of 23 mantissa bits stay
-    float q = fminf(__uint_as_float(bits) - low, 448.0f);
+    float q = __uint_as_float(min(bits, 0x43e00000u)) - low;      // at most 448, NaN too (its block's scale is not finite)
     if (floor && t > 0.0f) q = fmaxf(q, 0x1p-9f);
     return q;
 }
@@ -265,7 +269,8 @@ __device__ __forceinline__ void aw_tile(const hrf_adamw_tensor& T, int64_t begin
             aw_scale(aw_wave_max(am), sm, im);
             aw_scale(aw_wave_max(ar), sr, ir);
             float qm[4], qr[4];
-            const uint32_t mixed = S.seed ^ hrf_mix32((uint32_t)((uint64_t)s >> 32));
+            // (a wavefront's block of 256 lies on one side of any multiple of 2^32)
+            const uint32_t mixed = S.seed ^ hrf_mix32((uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)s >> 32)));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t h = hrf_mix32(((uint32_t)s + k) ^ mixed);
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(256) void k_adamw(const hrf_adamw_tensor* __restric
         ++tile;
         if (tile < tile_end) which = tile_tensor[tile];     // (the next tile's tensor is on its way while this one is stepped)
         if (!T.grad) continue;          // no gradient this time: value, moments and step count stay
-        const int pk = T.kind & 3, gk = (T.kind >> 2) & 3;
+        const int gk = (T.kind >> 2) & 3;
         if (skip) {
             if (C.zero_grad) {
                 if (gk == AW_F32) aw_zero_tile<AW_F32>(T, begin);
@@ -336,9 +341,7 @@ __global__ __launch_bounds__(256) void k_adamw(const hrf_adamw_tensor* __restric
             S.inv_bc2 = (float)(1.0 / sqrt(1.0 - aw_pow(C.beta2, t)));
             S.seed = hrf_mix32(C.seed ^ hrf_mix32((uint32_t)t));
         }
-        const uintptr_t align = ((uintptr_t)T.param & (pk == AW_F32 ? 15u : 7u)) | ((uintptr_t)T.grad & (gk == AW_F32 ? 15u : 7u)) |
-                                ((uintptr_t)T.copy & 7u);
-        const bool full = align == 0 && begin + AW_TILE <= T.n;
+        const bool full = begin + AW_TILE <= T.n;
 #define AW_CASE(P, G)                                                                                        \
     case (P) | ((G) << 2):                                                                                   \
         if (full) aw_tile<kBits, P, G, true>(T, begin, C, S, exp_avg, second, exp_avg_scale, second_scale);  \
@@ -394,7 +397,9 @@ __global__ __launch_bounds__(kThreads) void k_grad_norm(const hrf_adamw_tensor* 
                                                         const hrf_grad_scaler* __restrict__ scaler, float* __restrict__ out)
 {
     double sum = 0.0;
-    const int thread = threadIdx.x & 255, first = blockIdx.x * (kThreads / 256) + (threadIdx.x >> 8), stride = gridDim.x * (kThreads / 256);
+    // (a wavefront's tile is a scalar: a vector's worth of descriptors costs a fifth of the bandwidth)
+    const int thread = kThreads == 256 ? (int)threadIdx.x : (int)(threadIdx.x & 255), stride = kThreads == 256 ? (int)gridDim.x : kThreads / 256;
+    const int first = kThreads == 256 ? (int)blockIdx.x : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 8));
     int which = first < num_tiles ? tile_tensor[first] : 0;
     for (int tile = first; tile < num_tiles;) {
         const void* grad = tensors[which].grad;
@@ -404,14 +409,14 @@ __global__ __launch_bounds__(kThreads) void k_grad_norm(const hrf_adamw_tensor* 
         if (tile < num_tiles) which = tile_tensor[tile];
         if (!grad) continue;
         float g[8];
-        if (((uintptr_t)grad & 15u) == 0 && begin + AW_TILE <= n) {
+        if (begin + AW_TILE <= n) {
             if (gk == AW_F32) {
-                const AW_GLOBAL aw_f4* p = (const AW_GLOBAL aw_f4*)((const float*)grad + begin) + thread;
+                const AW_GLOBAL aw_f4u* p = (const AW_GLOBAL aw_f4u*)((const float*)grad + begin) + thread;
                 const aw_f4 x = p[0], y = p[256];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) { g[k] = x[k]; g[4 + k] = y[k]; }
             } else {
-                const aw_u4 x = *((const AW_GLOBAL aw_u4*)((const uint16_t*)grad + begin) + thread);
+                const aw_u4 x = *((const AW_GLOBAL aw_u4u*)((const uint16_t*)grad + begin) + thread);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) g[k] = aw_widen16((x[k >> 1] >> (16 * (k & 1))) & 0xffffu, gk == AW_BF16);
             }

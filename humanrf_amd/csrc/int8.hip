@@ -228,7 +228,7 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
     tn = in / height;
 }
 
-// Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 64
+// Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 64 R
 // bytes of k in LDS, four stages, filled by direct loads (16 bytes a lane, no registers) three stages ahead. W's packed blocks lie there as
 // in memory: 16 lanes that read together read 256 bytes side by side. A token's four 16-byte chunks lie permuted by its number, so that 16
 // lanes that read the same chunk of neighbouring tokens hit all 64 banks.
@@ -237,11 +237,12 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 // to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
 // LDS is what bounds smaller tiles. 8192^3: 897 us with 128 x 128 tiles, 483 us (2.27 POP/s) with 256 x 256; the library's product of
 // the same integers reaches 2.14.
-template <int K, int TM, int TN>
+template <int K, int TM, int TN, int R>
 __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const I8Args A)
 {
-    constexpr int BM = 64 * TM, BN = 64 * TN, kStage = (BM + BN) * 64, kLoads = (BM + BN) / 64;      // loads of a wavefront a stage
-    constexpr int kGroups = kLoads / 2, kReads = (TM + TN) / kGroups, kProducts = TM * TN / kGroups;
+    constexpr int BM = 64 * TM, BN = 64 * TN, kRun = (BM + BN) * 64, kStage = kRun * R;
+    constexpr int kPerRun = (BM + BN) / 64, kLoads = kPerRun * R;       // loads of a wavefront: of 64 bytes of k, of a stage
+    constexpr int kGroups = kLoads / 2, kReads = (TM + TN) * R / kGroups, kProducts = TM * TN * R / kGroups;
     typedef typename I8Type<K>::T T;
     typedef int i8_v16 __attribute__((ext_vector_type(16)));
     __shared__ __align__(16) int8_t s_tile[4 * kStage];
@@ -250,19 +251,22 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
     int tm, tn;
     i8_tile_of((A.rows + BM - 1) / BM, (A.cols + BN - 1) / BN, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int steps = A.inner >> 6;
+    const int steps = A.inner / (64 * R);
 
     // Load i of the wavefronts 0, 1: 16 tokens, this lane's row lane / 4 of them (past the end: the last one), its chunk permuted.
     // Of the wavefronts 2, 3: a block of 16 channels (past the end: the last one).
-    uint32_t from[kLoads];
+    uint32_t from[kPerRun];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-        from[i] = wave < 2 ? (uint32_t)min((wave * kLoads + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
-                           : (uint32_t)(min((n0 >> 4) + (wave - 2) * kLoads + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
+    for (int i = 0; i < kPerRun; ++i)
+        from[i] = wave < 2 ? (uint32_t)min((wave * kPerRun + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
+                           : (uint32_t)(min((n0 >> 4) + (wave - 2) * kPerRun + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
     const int8_t* const base = wave < 2 ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
     const int forward = wave < 2 ? 64 : 1024;
-    const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kLoads * 1024;
-    auto load = [&](int i, int s) { i8_load_lds(base + (int64_t)min(s, steps - 1) * forward, from[i], lds + (s & 3) * kStage + i * 1024); };
+    const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kPerRun * 1024;
+    auto load = [&](int i, int s) {
+        const int run = i / kPerRun, j = i % kPerRun;
+        i8_load_lds(base + ((int64_t)min(s, steps - 1) * R + run) * forward, from[j], lds + (s & 3) * kStage + run * kRun + j * 1024);
+    };
 
     i8_v16 acc[TN][TM];
 #pragma unroll
@@ -271,23 +275,24 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
         for (int b = 0; b < TM; ++b)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[a][b][k] = 0;
-    i8_v4 fr[2][TM + TN];       // two sets of operands: of the tokens, then of the channels
+    i8_v4 fr[2][R * (TM + TN)]; // two sets of operands, half a stage each: for every 32 k of the tokens, then of the channels
     const int x_row = (wm * 32 * TM + (lane & 31)) * 64, w_row = (BM / 16 + wn * 2 * TN) * 1024 + ((lane >> 4) & 1) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
-    auto read = [&](int set, int j, int s, int kk) {
-        const int8_t* t = s_tile + (s & 3) * kStage;
-        if (j < TM) fr[set][j] = *(const i8_v4*)(t + x_row + ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16 + j * 2048);
-        else fr[set][j] = *(const i8_v4*)(t + w_row + kk * 512 + (j - TM) * 2048);
+    auto read = [&](int set, int o, int s, int half) {
+        const int j = o % (TM + TN), kk = (half * R + o / (TM + TN)) & 1, run = (half * R + o / (TM + TN)) >> 1;
+        const int8_t* t = s_tile + (s & 3) * kStage + run * kRun;
+        if (j < TM) fr[set][o] = *(const i8_v4*)(t + x_row + ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16 + j * 2048);
+        else fr[set][o] = *(const i8_v4*)(t + w_row + kk * 512 + (j - TM) * 2048);
     };
-    // the products of one set, between them the reads of the other (k half `kk` of stage `next`) and half of the loads of stage `ahead`
-    auto work = [&](int set, int next, int kk, int ahead) {
+    // the products of one set, between them the reads of the other (a half of stage `next`) and half of the loads of stage `ahead`
+    auto work = [&](int set, int next, int half, int ahead) {
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-            for (int j = 0; j < kReads; ++j) read(set ^ 1, g * kReads + j, next, kk);
+            for (int j = 0; j < kReads; ++j) read(set ^ 1, g * kReads + j, next, half);
 #pragma unroll
             for (int p = 0; p < kProducts; ++p) {
-                const int a = (g * kProducts + p) / TM, b = (g * kProducts + p) % TM;
-                acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][TM + a], fr[set][b], acc[a][b], 0, 0, 0);
+                const int o = (g * kProducts + p) / (TM * TN) * (TM + TN), a = (g * kProducts + p) % (TM * TN) / TM, b = (g * kProducts + p) % TM;
+                acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][o + TM + a], fr[set][o + b], acc[a][b], 0, 0, 0);
             }
             load(set * kGroups + g, ahead);
             __builtin_amdgcn_sched_barrier(0);
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
         for (int i = 0; i < kLoads; ++i) load(i, s);
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
 #pragma unroll
-    for (int j = 0; j < TM + TN; ++j) read(0, j, 0, 0);
+    for (int j = 0; j < R * (TM + TN); ++j) read(0, j, 0, 0);
     for (int s = 0; s < steps; ++s) {
         work(0, s, 1, s + 3);
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + kGroups) : "memory");   // stage s + 1 has landed, of two more 3 halves are on their way
@@ -650,8 +655,13 @@ static void i8_pack(const int8_t* x, int64_t rows, int64_t cols, int64_t ldx, in
     hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, x, rows, (int)cols, ldx, packed, padded, pieces);
 }
 
-// Rows of up to 256 values and up to 128 channels, when there are enough rows to fill the card.
-static bool i8_is_short(int64_t rows, int64_t cols, int64_t padded) { return padded == 64 || (padded <= 256 && cols <= 128 && rows > 4096); }
+// Rows of up to 256 values, where rounding them first (a launch, codes written and read again) costs more than reading x once for every 64
+// channels. Captured calls, this way against the other: 100000 x 64 x 128 15 us against 50, 100000 x 128 x 256 46 against 72, 100000 x 256 x 256
+// 81 against 63; 4000 x 128 x 128 4.4 against 6.0, 2000 x 512 x 128 4.7 against 6.1. Rows of up to 64 have no other way.
+static bool i8_is_short(int64_t rows, int64_t cols, int64_t padded)
+{
+    return padded == 64 || (padded <= 256 && rows > 64 && (cols <= 192 || (cols <= 512 && rows <= 4096)));
+}
 
 template <int X, int K>
 static void i8_short(const I8Args& A, const I8Short& B, hipStream_t stream)
@@ -686,6 +696,13 @@ static void i8_few(const I8Args& A, hipStream_t stream)
     else hipLaunchKernelGGL((k_linear_i8_few<K, MT, NT, 4>), grid, dim3(256), 0, stream, A);
 }
 
+template <int K, int T, int R>
+static void i8_tiles(const I8Args& A, hipStream_t stream)
+{
+    const int64_t tiles = (int64_t)((A.rows + 64 * T - 1) / (64 * T)) * ((A.cols + 64 * T - 1) / (64 * T));
+    hipLaunchKernelGGL((k_linear_i8<K, T, T, R>), dim3((unsigned)tiles), dim3(256), 0, stream, A);
+}
+
 #define I8_FEW 64       // rows up to which the product of few tokens runs, on packed codes
 
 template <int K>
@@ -694,12 +711,15 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
     if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
     if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return; }
-    const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256);
-    if (large >= 200) hipLaunchKernelGGL((k_linear_i8<K, 4, 4>), dim3((unsigned)large), dim3(256), 0, stream, A);
-    else {
-        const int64_t tiles = (int64_t)((A.rows + 127) / 128) * ((A.cols + 127) / 128);
-        hipLaunchKernelGGL((k_linear_i8<K, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, stream, A);
-    }
+    // The largest tiles of which there are enough for the card: 256 x 256 do not wait for LDS, smaller ones take more of it for each product
+    // but a fourth of them each is a fourth of the time where most CUs would have none. Captured calls, rounding included: 8192^3
+    // 547 / 686 / 1010 us with 256 / 128 / 64, 1237 x 2827 x 5225 66 / 36 / 51, 303 x 2718 x 1318 32 / 14 / 10, 219 x 71 x 5967 67 / 27 / 16 (64 x 64
+    // with 128 bytes of k a stage; with 64 bytes 24). With few stages the ends count, of which a CU overlaps those of two smaller tiles:
+    // 8192 x 8192 x 512 90 us with 256, 81 with 128.
+    const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256), middle = (int64_t)((A.rows + 127) / 128) * ((A.cols + 127) / 128);
+    if (large >= 200 && A.inner >= 1024) i8_tiles<K, 4, 1>(A, stream);
+    else if (middle >= 200) i8_tiles<K, 2, 1>(A, stream);
+    else i8_tiles<K, 1, 2>(A, stream);
 }
 
 template <int K>
