@@ -468,6 +468,7 @@ extern "C" int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* t
     if (num_tiles == 0) return 0;
     HRF_CHECK_ARG(tensors && tile_tensor && exp_avg && second && ctl, "NULL argument");
     HRF_CHECK_ARG(state_bits == 32 || (exp_avg_scale && second_scale), "8-bit states need their scales");
+    HRF_CHECK_ARG((((uintptr_t)exp_avg | (uintptr_t)second) & 15u) == 0, "states must begin at multiples of 16 bytes");
     AwConst C;
     C.lr = lr; C.beta1 = beta1; C.beta2 = beta2;
     C.one_minus_b1 = (float)(1.0 - beta1); C.b2 = (float)beta2; C.one_minus_b2 = (float)(1.0 - beta2); C.eps = (float)eps;

@@ -228,20 +228,23 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
     tn = in / height;
 }
 
-// Tiles of BM = 64 TM tokens x BN = 64 TN channels, four wavefronts 2 x 2, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 64 R
+// Tiles of BM = 64 TM tokens x BN = 32 TN WN channels, 2 x WN wavefronts, 32 TM x 32 TN each from v_mfma_i32_32x32x32_i8. A stage is 64 R
 // bytes of k in LDS, four stages, filled by direct loads (16 bytes a lane, no registers) three stages ahead. W's packed blocks lie there as
 // in memory: 16 lanes that read together read 256 bytes side by side. A token's four 16-byte chunks lie permuted by its number, so that 16
 // lanes that read the same chunk of neighbouring tokens hit all 64 banks.
 // Everything is dealt out between the products: while the matrix cores work on 32 k, the operands of the next 32 are read from LDS and
 // a quarter of the loads of the third stage on is issued (sixteen loads in a row hold the wavefront up for as long as they take
 // to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
-// LDS is what bounds smaller tiles. 8192^3: 897 us with 128 x 128 tiles, 483 us (2.27 POP/s) with 256 x 256; the library's product of
-// the same integers reaches 2.14.
-template <int K, int TM, int TN, int R>
-__global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const I8Args A)
+// 8192^3 with 256 x 256 tiles: 478 us (2.30 POP/s; the library's product of the same integers reaches 2.14), the matrix cores at work 54 %
+// of the time at the 1.9 GHz that the card holds under this load, 417 us for every 8192 k more; the rest are the ends of the four tiles
+// each CU takes, where nothing is multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile,
+// took 505: the registers it needs are not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119.
+template <int K, int TM, int TN, int WN, int R>
+__global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
 {
-    constexpr int BM = 64 * TM, BN = 64 * TN, kRun = (BM + BN) * 64, kStage = kRun * R;
-    constexpr int kPerRun = (BM + BN) / 64, kLoads = kPerRun * R;       // loads of a wavefront: of 64 bytes of k, of a stage
+    constexpr int BM = 64 * TM, BN = 32 * TN * WN, kThreads = 128 * WN, kRun = (BM + BN) * 64, kStage = kRun * R;
+    constexpr int kPerRun = (BM + BN) / (32 * WN), kLoads = kPerRun * R;       // loads of a wavefront: of 64 bytes of k, of a stage
+    static_assert(BM == BN && kLoads % 2 == 0, "half of the wavefronts load tokens, half channels");
     constexpr int kGroups = kLoads / 2, kReads = (TM + TN) * R / kGroups, kProducts = TM * TN * R / kGroups;
     typedef typename I8Type<K>::T T;
     typedef int i8_v16 __attribute__((ext_vector_type(16)));
@@ -253,15 +256,15 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
     const int m0 = tm * BM, n0 = tn * BN;
     const int steps = A.inner / (64 * R);
 
-    // Load i of the wavefronts 0, 1: 16 tokens, this lane's row lane / 4 of them (past the end: the last one), its chunk permuted.
-    // Of the wavefronts 2, 3: a block of 16 channels (past the end: the last one).
+    // Load i of the first half of the wavefronts: 16 tokens, this lane's row lane / 4 of them (past the end: the last one), its chunk permuted.
+    // Of the second half: a block of 16 channels (past the end: the last one).
     uint32_t from[kPerRun];
 #pragma unroll
     for (int i = 0; i < kPerRun; ++i)
-        from[i] = wave < 2 ? (uint32_t)min((wave * kPerRun + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
-                           : (uint32_t)(min((n0 >> 4) + (wave - 2) * kPerRun + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
-    const int8_t* const base = wave < 2 ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
-    const int forward = wave < 2 ? 64 : 1024;
+        from[i] = wave < WN ? (uint32_t)min((wave * kPerRun + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
+                           : (uint32_t)(min((n0 >> 4) + (wave - WN) * kPerRun + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
+    const int8_t* const base = wave < WN ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
+    const int forward = wave < WN ? 64 : 1024;
     const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kPerRun * 1024;
     auto load = [&](int i, int s) {
         const int run = i / kPerRun, j = i % kPerRun;
@@ -298,8 +301,8 @@ __global__ __launch_bounds__(256, (TM * TN > 8 ? 1 : 2)) void k_linear_i8(const 
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    for (int k = threadIdx.x; k < BM; k += 256) s_sx[k] = A.sx[min(m0 + k, A.rows - 1)];
-    for (int k = threadIdx.x; k < BN; k += 256) {
+    for (int k = threadIdx.x; k < BM; k += kThreads) s_sx[k] = A.sx[min(m0 + k, A.rows - 1)];
+    for (int k = threadIdx.x; k < BN; k += kThreads) {
         const int n = min(n0 + k, A.cols - 1);
         s_sw[k] = A.sw[n];
         s_bias[k] = A.bias ? A.bias[n] : 0.0f;
@@ -696,11 +699,11 @@ static void i8_few(const I8Args& A, hipStream_t stream)
     else hipLaunchKernelGGL((k_linear_i8_few<K, MT, NT, 4>), grid, dim3(256), 0, stream, A);
 }
 
-template <int K, int T, int R>
+template <int K, int TM, int TN, int WN, int R>
 static void i8_tiles(const I8Args& A, hipStream_t stream)
 {
-    const int64_t tiles = (int64_t)((A.rows + 64 * T - 1) / (64 * T)) * ((A.cols + 64 * T - 1) / (64 * T));
-    hipLaunchKernelGGL((k_linear_i8<K, T, T, R>), dim3((unsigned)tiles), dim3(256), 0, stream, A);
+    const int64_t tiles = (int64_t)((A.rows + 64 * TM - 1) / (64 * TM)) * ((A.cols + 64 * TM - 1) / (64 * TM));
+    hipLaunchKernelGGL((k_linear_i8<K, TM, TN, WN, R>), dim3((unsigned)tiles), dim3(128 * WN), 0, stream, A);
 }
 
 #define I8_FEW 64       // rows up to which the product of few tokens runs, on packed codes
@@ -711,15 +714,15 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
     if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
     if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return; }
-    // The largest tiles of which there are enough for the card: 256 x 256 do not wait for LDS, smaller ones take more of it for each product
-    // but a fourth of them each is a fourth of the time where most CUs would have none. Captured calls, rounding included: 8192^3
-    // 547 / 686 / 1010 us with 256 / 128 / 64, 1237 x 2827 x 5225 66 / 36 / 51, 303 x 2718 x 1318 32 / 14 / 10, 219 x 71 x 5967 67 / 27 / 16 (64 x 64
-    // with 128 bytes of k a stage; with 64 bytes 24). With few stages the ends count, of which a CU overlaps those of two smaller tiles:
-    // 8192 x 8192 x 512 90 us with 256, 81 with 128.
+    // The largest tiles of which there are enough for the card: larger ones read each operand less often, but where most CUs would have none,
+    // smaller ones are done sooner. Captured calls, rounding included: 8192^3 517 / 681 / 1010 us with 256 / 128 / 64,
+    // 1237 x 2827 x 5225 63 / 36 / 51, 303 x 2718 x 1318 25 / 14 / 10, 219 x 71 x 5967 60 / 27 / 16 (64 x 64 with 128 bytes of k a stage; with 64
+    // bytes 24). With few stages the ends count, of which a CU overlaps those of two smaller tiles: 6465 x 1799 x 214 23.4 us
+    // with 256, 21.7 with 128, but 8192 x 8192 x 512 78 and 83.
     const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256), middle = (int64_t)((A.rows + 127) / 128) * ((A.cols + 127) / 128);
-    if (large >= 200 && A.inner >= 1024) i8_tiles<K, 4, 1>(A, stream);
-    else if (middle >= 200) i8_tiles<K, 2, 1>(A, stream);
-    else i8_tiles<K, 1, 2>(A, stream);
+    if (large >= 200 && A.inner >= 512) i8_tiles<K, 4, 2, 4, 1>(A, stream);
+    else if (middle >= 200) i8_tiles<K, 2, 2, 2, 1>(A, stream);
+    else i8_tiles<K, 1, 1, 2, 2>(A, stream);
 }
 
 template <int K>

@@ -610,6 +610,13 @@ def _on_device(device: torch.device):
     return _NOSPAN if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _disjoint(tensors, what: str) -> None:
+    """No two of the tensors share memory: workgroups step them side by side."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t is not None and t.numel() > 0)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise RuntimeError(f"AdamWPlan: two {what} share memory")
+
+
 _ADAMW_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -656,6 +663,7 @@ class AdamWPlan:
                 raise RuntimeError("AdamWPlan: copies are float16 or bfloat16 copies of float32 parameters")
             if c.numel() != p.numel() or c.device != p.device:
                 raise RuntimeError("AdamWPlan: a copy has its parameter's length and device")
+        _disjoint(params + copies, "parameters or copies")
         self.params, self.copies, self.state_bits, self.seed = params, copies, int(state_bits), int(seed) & 0xFFFFFFFF
         self.device = params[0].device
         self.lr_scales = [1.0] * len(params) if lr_scales is None else [float(x) for x in lr_scales]
@@ -720,6 +728,7 @@ class AdamWPlan:
                 raise RuntimeError(f"AdamWPlan: gradients must be float32, float16 or bfloat16, got {g.dtype}")
             if g.numel() != p.numel() or g.device != p.device:
                 raise RuntimeError("AdamWPlan: a gradient has its parameter's length and device")
+        _disjoint(grads, "gradients")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: the gradients' addresses change inside the capture of a graph; keep them in place "
                                "(zero them instead of dropping them) and set them before the capture")

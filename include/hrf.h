@@ -528,7 +528,8 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
  * the reference, whose optimizer is torch.optim.Adam on fp32 tensors (humanrf/run.py:101).
  * tensors: DEVICE array of `count` descriptors; tile_tensor: DEVICE int32[num_tiles], the tensor of each tile of 2048 elements, the
  * tiles of tensor k being first_tile .. first_tile + ceil(n / 2048) - 1.
- * States lie in flat buffers, tensor k's from position `base` (a multiple of 256) on, each tensor padded with zeros to whole blocks
+ * No two tensors share memory, nor do two copies or two gradients.
+ * States lie in flat buffers (at multiples of 16 bytes), tensor k's from position `base` (a multiple of 256) on, each tensor padded with zeros to whole blocks
  * of 256:
  *   state_bits 32: exp_avg, second = fp32 moments m and v;
  *   state_bits 8:  exp_avg, second = e4m3 (OCP fn) codes of m and of sqrt(v), exp_avg_scale / second_scale = fp32, one per block. Codes

@@ -22,7 +22,7 @@ def _adamw(lib, **change):
     (dict(weight_decay=float("inf")), b"hyper"), (dict(weight_decay=-1.0), b"hyper"), (dict(grad_scale=0.0), b"hyper"),
     (dict(eps=0.0), b"eps"), (dict(eps=1e-40), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(max_norm=1.0), b"norm"),
     (dict(tensors=None), b"NULL"), (dict(tile_tensor=None), b"NULL"), (dict(exp_avg=None), b"NULL"), (dict(second=None), b"NULL"),
-    (dict(ctl=None), b"NULL"), (dict(state_bits=8), b"scales"), (dict(state_bits=8, exp_avg_scale=FAKE), b"scales"),
+    (dict(ctl=None), b"NULL"), (dict(exp_avg=FAKE + 4), b"multiples of 16"), (dict(second=FAKE + 8), b"multiples of 16"), (dict(state_bits=8), b"scales"), (dict(state_bits=8, exp_avg_scale=FAKE), b"scales"),
 ])
 def test_the_step_refuses(change, said):
     from humanrf_amd import _lib

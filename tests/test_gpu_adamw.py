@@ -203,6 +203,43 @@ def test_factors_per_tensor(bits):
     del q
 
 
+def test_plans_refuse_on_the_device():
+    from humanrf_amd import ops
+    buf, g = torch.zeros(100, device="cuda"), torch.zeros(100, device="cuda")
+    for p in ([buf, buf], [buf[:60], buf[59:]]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.AdamWPlan(p)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.AdamWPlan([buf[:50], buf[50:]], [g[:50], g[:50]])
+    with pytest.raises(RuntimeError, match="length and device"):
+        ops.AdamWPlan([buf], [g[:99]])
+    with pytest.raises(RuntimeError, match="must be float32"):
+        ops.AdamWPlan([buf.double()])
+    with pytest.raises(RuntimeError, match="gradients must be"):
+        ops.AdamWPlan([buf], [g.double()])
+    with pytest.raises(RuntimeError, match="copies of float32"):
+        ops.AdamWPlan([buf.half()], copies=[g.half()])
+    with pytest.raises(RuntimeError, match="one gradient"):
+        ops.AdamWPlan([buf], [g, g])
+    with pytest.raises(RuntimeError, match="one finite factor"):
+        ops.AdamWPlan([buf], lr_scales=[-1.0])
+    plan = ops.AdamWPlan([buf], [g])
+    with pytest.raises(RuntimeError, match="state must hold"):
+        ops.AdamWPlan([buf], [g], state_bits=8, state=plan.state)
+    with pytest.raises(RuntimeError, match="must have 256 values"):
+        ops.AdamWPlan([buf], [g], state={k: v[:128] for k, v in plan.state.items()})
+    with pytest.raises(RuntimeError, match="max_norm"):
+        ops.adamw_multi(plan, LR, max_norm=1.0)
+    with pytest.raises(RuntimeError, match="max_norm"):
+        ops.adamw_multi(plan, LR, norm=ops.grad_norm_multi(plan), max_norm=0.0)
+    with pytest.raises(RuntimeError, match="not on the expected device"):
+        ops.adamw_multi(plan, LR, norm=torch.zeros(1))
+    with pytest.raises(RuntimeError, match="eps"):
+        ops.adamw_multi(plan, LR, eps=0.0)
+    with pytest.raises(RuntimeError, match="hyper"):
+        ops.adamw_multi(plan, LR, betas=(1.0, 0.9))
+
+
 def test_the_norm():
     from humanrf_amd import ops
     p, _ = _tensors((70_001, 3, 999_999), F32, 1)
