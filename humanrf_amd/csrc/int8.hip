@@ -235,10 +235,11 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 // Everything is dealt out between the products: while the matrix cores work on 32 k, the operands of the next 32 are read from LDS and
 // a quarter of the loads of the third stage on is issued (sixteen loads in a row hold the wavefront up for as long as they take
 // to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
-// 8192^3 with 256 x 256 tiles: 478 us (2.30 POP/s; the library's product of the same integers reaches 2.14), the matrix cores at work 54 %
-// of the time at the 1.9 GHz that the card holds under this load, 417 us for every 8192 k more; the rest are the ends of the four tiles
-// each CU takes, where nothing is multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile,
-// took 505: the registers it needs are not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119.
+// 8192^3 with 256 x 256 tiles: 478 us (2.30 POP/s; the library's product of the same integers reaches 2.14), bound by power: the matrix
+// cores are at work 73 % of the clocks, of which the card makes 1.5 GHz under this load (random codes; with zeros a tenth less time). No
+// bank conflicts in LDS. Every 8192 k more take 417 us; the rest are the ends of the four tiles that each CU takes, where nothing is
+// multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505: the registers for that are
+// not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119.
 template <int K, int TM, int TN, int WN, int R>
 __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
 {

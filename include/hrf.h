@@ -43,6 +43,9 @@
  *   hrf_render_loss_fused    volume_rendering.py:123-145 + trainer.py:205-247 + their autograd: composite, loss and the composite's
  *                            backward of the training step in one launch
  *   hrf_adam_*               humanrf/run.py:101 (torch.optim.Adam, betas .9/.99, eps 1e-15) + GradScaler skip
+ *   hrf_adamw_multi, hrf_grad_norm_multi  (no counterpart: decoupled weight decay, 8-bit states, clipping by the global norm, for callers
+ *                            that keep the reference's optimizer loop, humanrf/run.py:101)
+ *   hrf_linear_int8, hrf_int8_pack, hrf_quantize_rows_int8  (no counterpart: layers served with 8-bit weights, next to the fp16 networks)
  *   hrf_uniform_fill         torch.rand_like of humanrf/volume_rendering.py:63-64 (the stream hrf_prune_march draws from)
  *   hrf_occgrid_from_masks   actorshq/toolbox/native/occupancy_grid_generation.cu:16-120 (generate_from_masks)
  *   hrf_mask_dilate          actorshq/toolbox/generate_occupancy_grids_from_masks.py:64-77 (cv2.dilate of the masks)
