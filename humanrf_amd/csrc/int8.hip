@@ -109,15 +109,28 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
     }
 }
 
-// Codes that do not begin at multiples of 8 bytes, and rows too long for the registers: value by value, twice.
+// Rows too long for the registers: read twice, the second time from the cache. Also codes at any address.
 template <int K, bool kPacked>
-__global__ __launch_bounds__(256) void k_quantize_rows_any(const typename I8Type<K>::T* __restrict__ x, int64_t cols, int64_t ldx,
-                                                           int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
+__global__ __launch_bounds__(256) void k_quantize_rows_long(const typename I8Type<K>::T* __restrict__ x, int cols, int64_t ldx,
+                                                            int8_t* __restrict__ q, int ldq, float* __restrict__ scale)
 {
     __shared__ uint32_t s_max[4];
-    x += (int64_t)blockIdx.x * ldx;
+    constexpr int n = I8Piece<K>::n;
+    const typename I8Type<K>::T* const from = x + (int64_t)blockIdx.x * ldx;
+    auto get = [&](int k0, I8Piece<K>& v) {
+        if (k0 + n <= cols) i8_get<K>(v, from + k0);
+        else {
+#pragma unroll
+            for (int k = 0; k < n; ++k) v.v[k] = k0 + k < cols ? from[k0 + k] : I8Type<K>::down(0.0f);
+        }
+    };
     uint32_t top = 0;
-    for (int64_t k = threadIdx.x; k < cols; k += 256) top = max(top, i8_bits(I8Type<K>::up(x[k])));
+    for (int k0 = threadIdx.x * n; k0 < cols; k0 += 256 * n) {
+        I8Piece<K> v;
+        get(k0, v);
+#pragma unroll
+        for (int k = 0; k < n; ++k) top = max(top, i8_bits(I8Type<K>::up(v.v[k])));
+    }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
@@ -127,8 +140,20 @@ __global__ __launch_bounds__(256) void k_quantize_rows_any(const typename I8Type
     const float factor = i8_factor(top, sc);
     const bool finite = top < 0x7f800000u;
     if (threadIdx.x == 0) scale[blockIdx.x] = sc;
-    for (int k = threadIdx.x; k < (int)ldq; k += 256)
-        q[i8_at<kPacked>(blockIdx.x, k, ldq)] = k < cols ? (int8_t)i8_code(I8Type<K>::up(x[k]), factor, finite) : (int8_t)0;
+    for (int k0 = threadIdx.x * n; k0 < ldq; k0 += 256 * n) {
+        I8Piece<K> v;
+        get(k0, v);
+        int8_t* const to = q + i8_at<kPacked>(blockIdx.x, k0, ldq);
+        int8_t code[n];
+#pragma unroll
+        for (int k = 0; k < n; ++k) code[k] = (int8_t)i8_code(I8Type<K>::up(v.v[k]), factor, finite);
+        if (k0 + n <= ldq) __builtin_memcpy(to, code, n);
+        else {
+#pragma unroll
+            for (int k = 0; k < n; ++k)
+                if (k0 + k < ldq) to[k] = code[k];
+        }
+    }
 }
 
 // Rows of codes -> rows padded with zeros to ldq, a multiple of 16 bytes.
@@ -635,10 +660,10 @@ static void i8_quantize(const void* xv, int64_t rows, int64_t cols, int64_t ldx,
     hipLaunchKernelGGL((k_quantize_rows<K, kPacked, G, P>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))), dim3(256), 0, stream, x, rows, \
                        (int)cols, ldx, q, ldq, scale)
     if (!pieces || ldq > 256 * 8 * n)
-        hipLaunchKernelGGL((k_quantize_rows_any<K, kPacked>), dim3((unsigned)rows), dim3(256), 0, stream, x, cols, ldx, q, ldq, scale);
+        hipLaunchKernelGGL((k_quantize_rows_long<K, kPacked>), dim3((unsigned)rows), dim3(256), 0, stream, x, (int)cols, ldx, q, (int)ldq, scale);
     else if (ldq <= 16 * n) I8_ROWS(16, 1);
     else if (ldq <= 64 * n) I8_ROWS(64, 1);
-    else if (ldq <= 64 * 4 * n && !kPacked) I8_ROWS(64, 4);
+    else if (ldq <= 64 * 4 * n) I8_ROWS(64, 4);
     else if (ldq <= 256 * 2 * n) I8_ROWS(256, 2);
     else if (ldq <= 256 * 4 * n) I8_ROWS(256, 4);
     else I8_ROWS(256, 8);

@@ -88,6 +88,8 @@ class AdamW(torch.optim.Optimizer):
             plan.params, plan.lr_scales, plan.decay_scales = [p.detach() for p in params], lr_scales, decay_scales
             for p in plan.params:
                 ops._chk(p, "parameter")
+                if p.device != plan.device:
+                    raise RuntimeError("AdamW: the parameters have moved to another device after the first step")
             plan.set_grads(grads)
             plan.grads = None            # (held by the parameters; a second reference here would keep dropped gradients alive)
             self._key = key

@@ -132,7 +132,7 @@ def _check(sizes, bits, p0, g, p, copies, before, plan, factor, t, pdt):
 
 SIZES = (1, 255, 256, 257, 2047, 0, 2048, 2049, 7, 10_001)
 TYPES = [(F32, F32, None), (F32, F32, F16), (F32, BF16, BF16), (F32, F16, None), (BF16, BF16, None), (BF16, F32, None), (F16, F16, None),
-         (F16, F32, None)]
+         (F16, F32, None), (F16, BF16, None), (BF16, F16, None)]
 
 
 @pytest.mark.parametrize("offset", [0, 1, 2])

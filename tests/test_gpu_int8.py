@@ -40,7 +40,7 @@ def _holds(y, x, w, sx, sw, b, relu):
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 257, 65), (1, 130, 2051), (1, 4096, 1024), (2, 3, 127), (3, 200, 136), (5, 64, 5000), (8, 1000, 128), (9, 33, 64), (15, 65, 129),
           (16, 16, 1000), (17, 48, 128), (29, 520, 640), (31, 130, 64), (32, 257, 256), (33, 31, 300), (48, 1024, 512), (63, 100, 64), (64, 2048, 1024),
           (65, 63, 200), (100, 1500, 384), (127, 129, 1000), (128, 128, 128), (129, 257, 64), (255, 255, 255), (256, 512, 1024), (300, 130, 2051), (513, 1030, 640),
-          (1000, 64, 64), (1021, 515, 900), (4099, 64, 63), (5000, 17, 30), (5000, 190, 250), (4200, 200, 129), (70, 500, 200), (100, 520, 100), (20_000, 100, 64), (1300, 2050, 256), (2100, 2300, 1024)]
+          (1000, 64, 64), (1021, 515, 900), (4099, 64, 63), (5000, 17, 30), (5000, 190, 250), (4200, 200, 129), (70, 500, 200), (100, 520, 100), (20_000, 100, 64), (1300, 2050, 256), (3, 40, 20_001), (70, 30, 17_000), (2100, 2300, 1024)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -173,6 +173,21 @@ def test_refusals_on_the_device():
         ops.quantize_int8(torch.zeros(2, 131072, device="cuda"))
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
         ops.quantize_int8(x)
+
+
+def test_codes_at_any_address():
+    """The C entry writes codes with any row stride, at any address, and zeros from the row's end to the stride."""
+    from humanrf_amd import _lib, ops
+    from humanrf_amd._lib import check, ptr, stream_ptr
+    for dtype, kind in ((F32, 0), (F16, 1), (BF16, 2)):
+        for m, k, ld, at in ((5, 77, 77, 1), (5, 77, 83, 3), (3, 20_001, 20_003, 5), (9, 130, 136, 8)):
+            x = torch.randn(m, k, device="cuda").to(dtype)
+            q, s = ops.quantize_int8(x)
+            buf, scale = torch.full((m * ld + 64,), 99, dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda")
+            check(_lib.lib().hrf_quantize_rows_int8(ptr(x), kind, m, k, k, buf.data_ptr() + at, ld, ptr(scale), stream_ptr()))
+            got = buf[at:at + m * ld].view(m, ld)
+            assert torch.equal(got[:, :k], q) and int(got[:, k:].abs().sum()) == 0 and torch.equal(scale, s)
+            assert bool((buf[:at] == 99).all()) and bool((buf[at + m * ld:] == 99).all())
 
 
 def test_packed_codes():
