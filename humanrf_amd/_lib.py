@@ -37,13 +37,6 @@ class AdamTensor(ctypes.Structure):
                 ("group", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
-class AdamWTensor(ctypes.Structure):
-    """hrf_adamw_tensor (include/hrf.h)."""
-    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("copy", ctypes.c_void_p), ("n", ctypes.c_int64),
-                ("base", ctypes.c_int64), ("first_tile", ctypes.c_int32), ("kind", ctypes.c_int32),
-                ("lr_scale", ctypes.c_double), ("decay_scale", ctypes.c_double)]
-
-
 class GradScaler(ctypes.Structure):
     """hrf_grad_scaler (include/hrf.h)."""
     _fields_ = [("scale", ctypes.c_float), ("growth_factor", ctypes.c_float), ("backoff_factor", ctypes.c_float),

@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -618,6 +619,8 @@ def _disjoint(tensors, what: str) -> None:
 
 
 _ADAMW_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ADAMW_TENSOR = np.dtype([("param", "u8"), ("grad", "u8"), ("copy", "u8"), ("n", "i8"), ("base", "i8"), ("first_tile", "i4"), ("kind", "i4"),
+                          ("lr_scale", "f8"), ("decay_scale", "f8")])      # hrf_adamw_tensor (include/hrf.h)
 
 
 class AdamWPlan:
@@ -671,26 +674,24 @@ class AdamWPlan:
         for scales in (self.lr_scales, self.decay_scales):
             if len(scales) != len(params) or not all(0.0 <= x < float("inf") for x in scales):
                 raise RuntimeError("AdamWPlan: one finite factor >= 0 for each parameter")
-        self.offsets, self._first_tile, tiles, at, count = [], [], [], 0, 0
-        for k, p in enumerate(params):
-            self.offsets.append(at)
-            self._first_tile.append(count)
-            here = -(-p.numel() // self.TILE)
-            tiles.append(here)
-            count += here
-            at += -(-p.numel() // self.BLOCK) * self.BLOCK
-        self.numel, self.num_tiles = at, count
+        lengths = np.array([p.numel() for p in params], dtype=np.int64)
+        blocks, tiles = -(-lengths // self.BLOCK), -(-lengths // self.TILE)
+        self.offsets = [int(x) for x in (np.cumsum(blocks) - blocks) * self.BLOCK]
+        self.numel, self.num_tiles = int(blocks.sum()) * self.BLOCK, int(tiles.sum())
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: build the plan before the capture of a graph")
+        self._rows = np.zeros(len(params), dtype=_ADAMW_TENSOR)
+        self._rows["n"], self._rows["base"], self._rows["first_tile"] = lengths, self.offsets, np.cumsum(tiles) - tiles
         self.state = self._take_state(state)
-        self._ctl = torch.zeros(_lib.ADAMW_CTL + len(params), dtype=torch.int32, device=self.device)
-        if step:
-            self._ctl[_lib.ADAMW_CTL:] = int(step)
-        self._tile_tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), torch.tensor(tiles)).to(self.device)
-        self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
-        self._desc = None
-        self.grads = None
+        with _on_device(self.device):
+            self._ctl = torch.zeros(_lib.ADAMW_CTL + len(params), dtype=torch.int32, device=self.device)
+            if step:
+                self._ctl[_lib.ADAMW_CTL:] = int(step)
+            self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
+        self.grads, self._desc = None, None
+        self._tiles = np.repeat(np.arange(len(params), dtype=np.int32), tiles)
         self.set_grads([None] * len(params) if grads is None else grads)
+        del self._tiles
         # what the entry points take of the plan, as addresses: none of these buffers is ever replaced
         st = list(self.state.values())
         first, second, scales = (st[0], st[1], (None, None)) if self.state_bits == 32 else (st[0], st[2], (st[1], st[3]))
@@ -732,17 +733,19 @@ class AdamWPlan:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: the gradients' addresses change inside the capture of a graph; keep them in place "
                                "(zero them instead of dropping them) and set them before the capture")
-        arr = (_lib.AdamWTensor * len(grads))()
-        for k, (p, g, c) in enumerate(zip(self.params, grads, self.copies)):
-            kind = _ADAMW_KINDS[p.dtype] | (_ADAMW_KINDS[g.dtype] << 2 if g is not None else 0) | (_ADAMW_KINDS[c.dtype] << 4 if c is not None else 0)
-            # (an empty tensor has no storage, but it has a gradient: its step count advances)
-            arr[k] = _lib.AdamWTensor(ptr(p), None if g is None else (ptr(g) or 1), ptr(c), p.numel(), self.offsets[k], self._first_tile[k], kind,
-                                      self.lr_scales[k], self.decay_scales[k])
-        host = torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).pin_memory()
+        rows = self._rows
+        rows["param"], rows["copy"] = [p.data_ptr() for p in self.params], [0 if c is None else c.data_ptr() for c in self.copies]
+        # (an empty tensor has no storage, but it has a gradient: its step count advances)
+        rows["grad"] = [0 if g is None else (g.data_ptr() or 1) for g in grads]
+        rows["kind"] = [_ADAMW_KINDS[p.dtype] | (_ADAMW_KINDS[g.dtype] << 2 if g is not None else 0) | (_ADAMW_KINDS[c.dtype] << 4 if c is not None else 0)
+                        for p, g, c in zip(self.params, grads, self.copies)]
+        rows["lr_scale"], rows["decay_scale"] = self.lr_scales, self.decay_scales
         with _on_device(self.device):
-            if self._desc is None:
-                self._desc = torch.empty(host.numel(), dtype=torch.uint8, device=self.device)
-            self._desc.copy_(host, non_blocking=True)
+            if self._desc is None:      # the descriptors, and behind them the tensor of each tile
+                self._desc = torch.from_numpy(np.concatenate([rows.view(np.uint8), self._tiles.view(np.uint8)])).to(self.device)
+                self._tile_tensor = self._desc[rows.nbytes:]
+            else:
+                self._desc[:rows.nbytes].copy_(torch.from_numpy(rows.view(np.uint8)).pin_memory(), non_blocking=True)
         self.grads = grads
 
     @property

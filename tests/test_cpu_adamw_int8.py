@@ -1,7 +1,5 @@
 """What the AdamW step and the 8-bit integer product refuse, on the CPU: through the C entry points (arguments are looked at before
 anything is launched) and through the Python wrappers."""
-import ctypes
-
 import pytest
 import torch
 
@@ -50,10 +48,11 @@ def test_the_norm_refuses(args):
 
 
 def test_the_descriptor_has_the_header_s_layout():
-    from humanrf_amd import _lib
-    D = _lib.AdamWTensor
-    assert ctypes.sizeof(D) == 64
-    assert [getattr(D, f).offset for f in ("param", "grad", "copy", "n", "base", "first_tile", "kind", "lr_scale", "decay_scale")] == \
+    """The rows that the plan writes are hrf_adamw_tensor as a C compiler lays it out."""
+    from humanrf_amd import ops
+    D = ops._ADAMW_TENSOR
+    assert D.itemsize == 64
+    assert [D.fields[f][1] for f in ("param", "grad", "copy", "n", "base", "first_tile", "kind", "lr_scale", "decay_scale")] == \
         [0, 8, 16, 24, 32, 40, 44, 48, 56]
 
 
