@@ -260,18 +260,19 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 // Everything is dealt out between the products: while the matrix cores work on 32 k, the operands of the next 32 are read from LDS and
 // a quarter of the loads of the third stage on is issued (sixteen loads in a row hold the wavefront up for as long as they take
 // to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
-// 8192^3 with 256 x 256 tiles: 478 us (2.30 POP/s; the library's product of the same integers reaches 2.14), bound by power: the matrix
+// 8192^3 with 256 x 256 tiles: 469 us (2.34 POP/s; the library's product of the same integers reaches 2.14), bound by power: the matrix
 // cores are at work 73 % of the clocks, of which the card makes 1.5 GHz under this load (random codes; with zeros a tenth less time). No
 // bank conflicts in LDS. Every 8192 k more take 417 us; the rest are the ends of the four tiles that each CU takes, where nothing is
-// multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505: the registers for that are
-// not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119.
+// multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505 where one tile a workgroup took 483: the registers for that are
+// not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119. 128 x 128 tiles are bound by what
+// the L2 gives, some 13 TB/s.
 template <int K, int TM, int TN, int WN, int R>
-__global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
+__global__ __launch_bounds__(128 * WN, (TM * TN * WN > 8 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
 {
     constexpr int BM = 64 * TM, BN = 32 * TN * WN, kThreads = 128 * WN, kRun = (BM + BN) * 64, kStage = kRun * R;
     constexpr int kPerRun = (BM + BN) / (32 * WN), kLoads = kPerRun * R;       // loads of a wavefront: of 64 bytes of k, of a stage
-    static_assert(BM == BN && kLoads % 2 == 0, "half of the wavefronts load tokens, half channels");
-    constexpr int kGroups = kLoads / 2, kReads = (TM + TN) * R / kGroups, kProducts = TM * TN * R / kGroups;
+    static_assert((BM + BN) % (32 * WN) == 0, "every wavefront loads as much");
+    constexpr int kOperands = R * (TM + TN), kProducts = R * TM * TN, kGroups = kProducts % 3 == 0 ? 3 : 2, kEarly = (kLoads + 1) / 2;
     typedef typename I8Type<K>::T T;
     typedef int i8_v16 __attribute__((ext_vector_type(16)));
     __shared__ __align__(16) int8_t s_tile[4 * kStage];
@@ -282,19 +283,23 @@ __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) voi
     const int m0 = tm * BM, n0 = tn * BN;
     const int steps = A.inner / (64 * R);
 
-    // Load i of the first half of the wavefronts: 16 tokens, this lane's row lane / 4 of them (past the end: the last one), its chunk permuted.
-    // Of the second half: a block of 16 channels (past the end: the last one).
+    // Load j of 64 bytes of k is number wave * kPerRun + j of the tile: first the tokens, 16 a load, this lane's row lane / 4 of them (past the
+    // end: the last one), its chunk permuted; then the channels, a block of 16 (past the end: the last one).
     uint32_t from[kPerRun];
 #pragma unroll
-    for (int i = 0; i < kPerRun; ++i)
-        from[i] = wave < WN ? (uint32_t)min((wave * kPerRun + i) * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
-                           : (uint32_t)(min((n0 >> 4) + (wave - WN) * kPerRun + i, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
-    const int8_t* const base = wave < WN ? A.x + (int64_t)m0 * A.ldx : A.w + (int64_t)n0 * A.inner;
-    const int forward = wave < WN ? 64 : 1024;
+    for (int j = 0; j < kPerRun; ++j) {
+        const int sixteen = wave * kPerRun + j;
+        from[j] = sixteen < BM / 16 ? (uint32_t)min(sixteen * 16 + (lane >> 2), A.rows - 1 - m0) * (uint32_t)A.ldx + ((lane & 3) ^ (lane >> 4)) * 16
+                                    : (uint32_t)(min((n0 >> 4) + sixteen - BM / 16, (A.cols - 1) >> 4) - (n0 >> 4)) * (uint32_t)A.inner * 16 + lane * 16;
+    }
+    const int8_t* const xb = A.x + (int64_t)m0 * A.ldx;
+    const int8_t* const wb = A.w + (int64_t)n0 * A.inner;
     const uint32_t lds = (uint32_t)(uintptr_t)(I8_LDS int8_t*)s_tile + wave * kPerRun * 1024;
     auto load = [&](int i, int s) {
         const int run = i / kPerRun, j = i % kPerRun;
-        i8_load_lds(base + ((int64_t)min(s, steps - 1) * R + run) * forward, from[j], lds + (s & 3) * kStage + run * kRun + j * 1024);
+        const int64_t at = (int64_t)min(s, steps - 1) * R + run;
+        const bool token = wave * kPerRun + j < BM / 16;
+        i8_load_lds((token ? xb : wb) + at * (token ? 64 : 1024), from[j], lds + (s & 3) * kStage + run * kRun + j * 1024);
     };
 
     i8_v16 acc[TN][TM];
@@ -314,16 +319,20 @@ __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) voi
     };
     // the products of one set, between them the reads of the other (a half of stage `next`) and half of the loads of stage `ahead`
     auto work = [&](int set, int next, int half, int ahead) {
+        const int first = set == 0 ? 0 : kEarly, loads = set == 0 ? kEarly : kLoads - kEarly;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-            for (int j = 0; j < kReads; ++j) read(set ^ 1, g * kReads + j, next, half);
+            for (int j = 0; j < kOperands; ++j)
+                if (j * kGroups / kOperands == g) read(set ^ 1, j, next, half);
 #pragma unroll
-            for (int p = 0; p < kProducts; ++p) {
-                const int o = (g * kProducts + p) / (TM * TN) * (TM + TN), a = (g * kProducts + p) % (TM * TN) / TM, b = (g * kProducts + p) % TM;
+            for (int p = g * kProducts / kGroups; p < (g + 1) * kProducts / kGroups; ++p) {
+                const int o = p / (TM * TN) * (TM + TN), a = p % (TM * TN) / TM, b = p % TM;
                 acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][o + TM + a], fr[set][o + b], acc[a][b], 0, 0, 0);
             }
-            load(set * kGroups + g, ahead);
+#pragma unroll
+            for (int i = 0; i < kEarly; ++i)
+                if (i < loads && i * kGroups / kEarly == g) load(first + i, ahead);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -342,7 +351,7 @@ __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 16 ? 1 : 2) * WN / 2) voi
     for (int j = 0; j < R * (TM + TN); ++j) read(0, j, 0, 0);
     for (int s = 0; s < steps; ++s) {
         work(0, s, 1, s + 3);
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + kGroups) : "memory");   // stage s + 1 has landed, of two more 3 halves are on their way
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads + kEarly) : "memory");   // stage s + 1 has landed, of two more 3 halves are on their way
         work(1, s + 1, 0, s + 3);       // (past the end: stages that are there, read again and not used)
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // nothing may land in LDS that is somebody else's by then
@@ -728,7 +737,7 @@ static void i8_few(const I8Args& A, hipStream_t stream)
 template <int K, int TM, int TN, int WN, int R>
 static void i8_tiles(const I8Args& A, hipStream_t stream)
 {
-    const int64_t tiles = (int64_t)((A.rows + 64 * TM - 1) / (64 * TM)) * ((A.cols + 64 * TM - 1) / (64 * TM));
+    const int64_t tiles = (int64_t)((A.rows + 64 * TM - 1) / (64 * TM)) * ((A.cols + 32 * TN * WN - 1) / (32 * TN * WN));
     hipLaunchKernelGGL((k_linear_i8<K, TM, TN, WN, R>), dim3((unsigned)tiles), dim3(128 * WN), 0, stream, A);
 }
 
@@ -740,14 +749,19 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
     if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
     if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return; }
-    // The largest tiles of which there are enough for the card: larger ones read each operand less often, but where most CUs would have none,
-    // smaller ones are done sooner. Captured calls, rounding included: 8192^3 517 / 681 / 1010 us with 256 / 128 / 64,
-    // 1237 x 2827 x 5225 63 / 36 / 51, 303 x 2718 x 1318 25 / 14 / 10, 219 x 71 x 5967 60 / 27 / 16 (64 x 64 with 128 bytes of k a stage; with 64
-    // bytes 24). With few stages the ends count, of which a CU overlaps those of two smaller tiles: 6465 x 1799 x 214 23.4 us
-    // with 256, 21.7 with 128, but 8192 x 8192 x 512 78 and 83.
-    const int64_t large = (int64_t)((A.rows + 255) / 256) * ((A.cols + 255) / 256), middle = (int64_t)((A.rows + 127) / 128) * ((A.cols + 127) / 128);
-    if (large >= 200 && A.inner >= 512) i8_tiles<K, 4, 2, 4, 1>(A, stream);
-    else if (middle >= 200) i8_tiles<K, 2, 2, 2, 1>(A, stream);
+    // Rounds of the card times what a round of that size takes against one of 128 x 128: larger tiles read each operand less often, smaller ones
+    // fill the card when there is little, and a round that only a few tiles need takes as long as a full one (264 tiles of 128 on 256
+    // CUs: two). Captured calls in us, rounding included, with 64 / 128 / 128 x 192 / 256:
+    //   219 x 71 x 5967   17 / 28 / 31 / 60      1237 x 2827 x 5225  50 / 35 / 39 / 63      1021 x 4099 x 2051  29 / 30 / 25 / 40
+    //   325 x 4341 x 6165 35 / 40 / 47 / 68      11905 x 625 x 1683  46 / 38 / 43 / 43      1000 x 5000 x 3000  39 / 34 / 30 / 43
+    //   4096^3           125 / 92 / 87 / 74      8192^3            1032 / 674 / 677 / 512   8192 x 8192 x 512  121 / 80 / 91 / 77
+    // (64 x 64 with 128 bytes of k a stage: with 64 bytes the first takes 24.) Below 512 k the ends count, which a CU overlaps for two
+    // of the smaller tiles: 6465 x 1799 x 214 27 / 21 / 24 / 23.
+    auto rounds = [&](int m, int n) { return (((int64_t)A.rows + m - 1) / m * (((int64_t)A.cols + n - 1) / n) + 255) / 256; };
+    const int64_t c64 = 9 * rounds(64, 64), c128 = 20 * rounds(128, 128), c192 = 25 * rounds(128, 192), c256 = 60 * rounds(256, 256);
+    if (A.inner >= 512 && c256 < std::min(std::min(c64, c128), c192)) i8_tiles<K, 4, 2, 4, 1>(A, stream);
+    else if (A.inner >= 512 && c192 < std::min(c64, c128)) i8_tiles<K, 2, 3, 2, 1>(A, stream);
+    else if (c128 < c64) i8_tiles<K, 2, 2, 2, 1>(A, stream);
     else i8_tiles<K, 1, 1, 2, 2>(A, stream);
 }
 

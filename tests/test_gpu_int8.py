@@ -40,7 +40,7 @@ def _holds(y, x, w, sx, sw, b, relu):
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 257, 65), (1, 130, 2051), (1, 4096, 1024), (2, 3, 127), (3, 200, 136), (5, 64, 5000), (8, 1000, 128), (9, 33, 64), (15, 65, 129),
           (16, 16, 1000), (17, 48, 128), (29, 520, 640), (31, 130, 64), (32, 257, 256), (33, 31, 300), (48, 1024, 512), (63, 100, 64), (64, 2048, 1024),
           (65, 63, 200), (100, 1500, 384), (127, 129, 1000), (128, 128, 128), (129, 257, 64), (255, 255, 255), (256, 512, 1024), (300, 130, 2051), (513, 1030, 640),
-          (1000, 64, 64), (1021, 515, 900), (4099, 64, 63), (5000, 17, 30), (5000, 190, 250), (4200, 200, 129), (70, 500, 200), (100, 520, 100), (20_000, 100, 64), (1300, 2050, 256), (3, 40, 20_001), (70, 30, 17_000), (2100, 2300, 1024)]
+          (1000, 64, 64), (1021, 515, 900), (4099, 64, 63), (5000, 17, 30), (5000, 190, 250), (4200, 200, 129), (70, 500, 200), (100, 520, 100), (20_000, 100, 64), (1300, 2050, 256), (3, 40, 20_001), (70, 30, 17_000), (2100, 2300, 1024), (1030, 4100, 600), (5000, 3000, 520)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
