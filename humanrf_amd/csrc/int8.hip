@@ -8,9 +8,9 @@
 // operand, so that a lane's results are neighbouring channels of one token.
 // W is packed: rows padded with zeros to 64 bytes (or a multiple of 128), cut into blocks of 16 rows x 64 bytes, a kilobyte
 // each, in which bytes 16 q .. 16 q + 15 of row t are the 16 bytes at 256 q + 16 t: what lane (t, q) of the first instruction takes. A
-// wavefront's load of an operand is then one kilobyte side by side. Few tokens are packed too; many stay rows, of which a stage of the
-// tiles reads 128 bytes each (rounding 8192 rows of 8192 straight into packed blocks takes 89 us, pieces of 16 bytes scattered by
-// different workgroups; into rows 35). 29 tokens x 10240 x 5120: both operands as rows, 16 pieces of 64 bytes a load, 31 us; packed 13.
+// wavefront's load of an operand is then one kilobyte side by side. Few tokens are packed too; many stay rows, of which the tiles read 64
+// bytes at a time (rounding 8192 rows of 8192 straight into packed blocks takes 89 us, pieces of 16 bytes scattered by different
+// workgroups; into rows 32). 29 tokens x 10240 x 5120: both operands as rows, 16 pieces of 64 bytes a load, 31 us; packed 13.
 // Epilogue in fp32, one rounding per operation, one to the type of y.
 #include "hrf_common.h"
 #include <algorithm>
@@ -54,7 +54,7 @@ __device__ __forceinline__ int64_t i8_at(int64_t row, int k, int64_t ld)
 }
 
 // kGroup lanes a row (a power of two up to a wavefront, or the whole workgroup of 256 joined through LDS). The row is read once, in 16-byte
-// pieces, and stays in registers, kPieces of them a lane. 8192 rows of 8192 bf16: 118 us read twice value by value, 35 us this way.
+// pieces, and stays in registers, kPieces of them a lane. 8192 rows of 8192 bf16: 118 us read twice value by value, 32 us this way.
 template <int K, bool kPacked, int kGroup, int kPieces>
 __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>::T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                             int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
@@ -263,9 +263,9 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 // 8192^3 with 256 x 256 tiles: 469 us (2.34 POP/s; the library's product of the same integers reaches 2.14), bound by power: the matrix
 // cores are at work 73 % of the clocks, of which the card makes 1.5 GHz under this load (random codes; with zeros a tenth less time). No
 // bank conflicts in LDS. Every 8192 k more take 417 us; the rest are the ends of the four tiles that each CU takes, where nothing is
-// multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505 where one tile a workgroup took 483: the registers for that are
-// not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us against 119. 128 x 128 tiles are bound by what
-// the L2 gives, some 13 TB/s.
+// multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505 us where one tile a
+// workgroup took 483: the registers for that are not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us
+// against 119. 128 x 128 tiles are bound by what the L2 gives, some 13 TB/s.
 template <int K, int TM, int TN, int WN, int R>
 __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 8 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
 {
