@@ -390,6 +390,26 @@ def test_captured_steps_on_another_stream(bits):
             assert plan.steps.tolist() == twin.steps.tolist() == [it + 2] * 2
 
 
+def test_two_plans_on_two_streams_at_once():
+    from humanrf_amd import ops
+
+    def make(k):
+        p, _ = _tensors((300_000, 5), F32, 30 + k)
+        g, _ = _tensors((300_000, 5), F32, 40 + k)
+        return ops.AdamWPlan(p, g, state_bits=8, seed=k)
+    plans, twins, streams = [make(0), make(1)], [make(0), make(1)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for plan, s in zip(plans, streams):
+            with torch.cuda.stream(s):
+                ops.adamw_multi(plan, LR, norm=ops.grad_norm_multi(plan), max_norm=1.0)
+    torch.cuda.synchronize()
+    for plan, twin in zip(plans, twins):
+        for _ in range(8):
+            ops.adamw_multi(twin, LR, norm=ops.grad_norm_multi(twin), max_norm=1.0)
+        assert all(torch.equal(a, b) for a, b in zip(plan.params, twin.params)) and plan.steps.tolist() == [8, 8]
+
+
 def test_offsets_past_32_bits():
     """A tensor of 2^31 + 777 values: its last block, and one at 2^31, are stepped as any other."""
     from humanrf_amd import ops

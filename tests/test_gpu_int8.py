@@ -260,6 +260,27 @@ def test_captured_products_on_another_stream(m):
         assert torch.equal(y, ops.linear_int8(x, h))
 
 
+def test_two_streams_at_once():
+    """One handle, calls of every kind interleaved on two streams: each has workspaces of its own."""
+    from humanrf_amd import ops
+    _, w, _, sw, b = _case(1, 200, 300)
+    h = ops.Int8Weight(w, sw, b)
+    xs = [torch.randn(m, 300, generator=_gen(m), device="cuda") for m in (1, 7, 40, 300, 1000)]
+    want = [ops.linear_int8(x, h) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for k in range(6):
+        for s, out in zip(streams, got):
+            with torch.cuda.stream(s):
+                out += [ops.linear_int8(x, h) for x in (xs if k % 2 else xs[::-1])]
+    torch.cuda.synchronize()
+    for out in got:
+        for k in range(6):
+            part = out[5 * k:5 * k + 5]
+            assert all(torch.equal(y, z) for y, z in zip(part if k % 2 else part[::-1], want))
+
+
 # ------------------------------------------------------------------------------------------------ modules, and all of it together
 def test_networks():
     """A layer of rounded weights and rows is off by half a step of each: sum_k |w| s_x / 2 + |x| s_w / 2 + s_x s_w / 4; a network's first
