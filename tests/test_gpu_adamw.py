@@ -507,9 +507,9 @@ def test_checkpoints(bits):
         assert torch.equal(od._plan.state["exp_avg_sq"], ob._plan.state["exp_avg_sq"]) and od._plan.steps.tolist() == [3] * 4
 
 
-def test_a_captured_training_step_while_an_eager_graph_of_its_leaves_lives():
-    """Forward, backward and step captured; an eager loss over the same leaves, with its autograd graph, is alive all the while and is
-    differentiated after the replays."""
+def test_a_captured_training_step():
+    """Forward, backward, norm and step captured and replayed, with eager steps of a twin between; an eager autograd graph over copies of
+    the parameters is alive all the while and is differentiated after the replays."""
     from humanrf_amd.optim import AdamW
     net, twin = _net(), _net()
     x, y = torch.randn(128, 24, device="cuda"), torch.randn(128, 3, device="cuda")
