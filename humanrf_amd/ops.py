@@ -649,24 +649,10 @@ class AdamWPlan:
             raise RuntimeError(f"AdamWPlan: state_bits must be 8 or 32, got {state_bits}")
         if int(step) < 0:
             raise RuntimeError("AdamWPlan: negative step count")
-        for p in params:
-            _chk(p, "parameter")
-            if p.dtype not in _ADAMW_KINDS:
-                raise RuntimeError(f"AdamWPlan: parameters must be float32, float16 or bfloat16, got {p.dtype}")
-            if p.device != params[0].device:
-                raise RuntimeError("AdamWPlan: the parameters lie on several devices")
         copies = [None] * len(params) if copies is None else list(copies)
         if len(copies) != len(params):
             raise RuntimeError("AdamWPlan: one copy (or None) for each parameter")
-        for p, c in zip(params, copies):
-            if c is None:
-                continue
-            _chk(c, "16-bit copy")
-            if p.dtype != torch.float32 or c.dtype not in (torch.float16, torch.bfloat16):
-                raise RuntimeError("AdamWPlan: copies are float16 or bfloat16 copies of float32 parameters")
-            if c.numel() != p.numel() or c.device != p.device:
-                raise RuntimeError("AdamWPlan: a copy has its parameter's length and device")
-        _disjoint(params + copies, "parameters or copies")
+        self._check_params(params, copies, params[0].device)
         self.params, self.copies, self.state_bits, self.seed = params, copies, int(state_bits), int(seed) & 0xFFFFFFFF
         self.device = params[0].device
         self.lr_scales = [1.0] * len(params) if lr_scales is None else [float(x) for x in lr_scales]
@@ -674,7 +660,8 @@ class AdamWPlan:
         for scales in (self.lr_scales, self.decay_scales):
             if len(scales) != len(params) or not all(0.0 <= x < float("inf") for x in scales):
                 raise RuntimeError("AdamWPlan: one finite factor >= 0 for each parameter")
-        lengths = np.array([p.numel() for p in params], dtype=np.int64)
+        self._lengths = [p.numel() for p in params]
+        lengths = np.array(self._lengths, dtype=np.int64)
         blocks, tiles = -(-lengths // self.BLOCK), -(-lengths // self.TILE)
         self.offsets = [int(x) for x in (np.cumsum(blocks) - blocks) * self.BLOCK]
         self.numel, self.num_tiles = int(blocks.sum()) * self.BLOCK, int(tiles.sum())
@@ -716,29 +703,62 @@ class AdamWPlan:
                 raise RuntimeError(f"AdamWPlan: state {name} must begin at a multiple of 16 bytes")
         return {name: state[name] for name in want}
 
+    @staticmethod
+    def _check_params(params, copies, device) -> None:
+        for p in params:
+            _chk(p, "parameter")
+            if p.dtype not in _ADAMW_KINDS:
+                raise RuntimeError(f"AdamWPlan: parameters must be float32, float16 or bfloat16, got {p.dtype}")
+            if p.device != device:
+                raise RuntimeError("AdamWPlan: the parameters lie on several devices")
+        for p, c in zip(params, copies):
+            if c is None:
+                continue
+            _chk(c, "16-bit copy")
+            if p.dtype != torch.float32 or c.dtype not in (torch.float16, torch.bfloat16):
+                raise RuntimeError("AdamWPlan: copies are float16 or bfloat16 copies of float32 parameters")
+            if c.numel() != p.numel() or c.device != p.device:
+                raise RuntimeError("AdamWPlan: a copy has its parameter's length and device")
+        _disjoint(params + copies, "parameters or copies")
+
+    def set_tensors(self, params, grads) -> None:
+        """Other storage for the parameters, each as long as the one it replaces (lengths, states and step counts are the plan's own), and
+        other gradients, as `set_grads`."""
+        params = list(params)
+        if len(params) != len(self.params):
+            raise RuntimeError("AdamWPlan: as many parameters as the plan was built over")
+        for k, (p, n) in enumerate(zip(params, self._lengths)):
+            if p.numel() != n:
+                raise RuntimeError(f"AdamWPlan: parameter {k} has {p.numel()} values, the plan was built over {n}: build another plan")
+        self._check_params(params, self.copies, self.device)
+        self._point_at(params, grads)
+
     def set_grads(self, grads) -> None:
         """Other gradient tensors (or None) for the next steps: the descriptors are written anew, on the current stream."""
+        self._point_at(self.params, grads)
+
+    def _point_at(self, params, grads) -> None:
         grads = list(grads)
-        if len(grads) != len(self.params):
+        if len(grads) != len(params):
             raise RuntimeError("AdamWPlan: one gradient (or None) for each parameter")
-        for p, g in zip(self.params, grads):
+        for n, g in zip(self._lengths, grads):
             if g is None:
                 continue
             _chk(g, "gradient")
             if g.dtype not in _ADAMW_KINDS:
                 raise RuntimeError(f"AdamWPlan: gradients must be float32, float16 or bfloat16, got {g.dtype}")
-            if g.numel() != p.numel() or g.device != p.device:
+            if g.numel() != n or g.device != self.device:
                 raise RuntimeError("AdamWPlan: a gradient has its parameter's length and device")
         _disjoint(grads, "gradients")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: the gradients' addresses change inside the capture of a graph; keep them in place "
                                "(zero them instead of dropping them) and set them before the capture")
         rows = self._rows
-        rows["param"], rows["copy"] = [p.data_ptr() for p in self.params], [0 if c is None else c.data_ptr() for c in self.copies]
+        rows["param"], rows["copy"] = [p.data_ptr() for p in params], [0 if c is None else c.data_ptr() for c in self.copies]
         # (an empty tensor has no storage, but it has a gradient: its step count advances)
         rows["grad"] = [0 if g is None else (g.data_ptr() or 1) for g in grads]
         rows["kind"] = [_ADAMW_KINDS[p.dtype] | (_ADAMW_KINDS[g.dtype] << 2 if g is not None else 0) | (_ADAMW_KINDS[c.dtype] << 4 if c is not None else 0)
-                        for p, g, c in zip(self.params, grads, self.copies)]
+                        for p, g, c in zip(params, grads, self.copies)]
         rows["lr_scale"], rows["decay_scale"] = self.lr_scales, self.decay_scales
         with _on_device(self.device):
             if self._desc is None:      # the descriptors, and behind them the tensor of each tile
@@ -746,7 +766,7 @@ class AdamWPlan:
                 self._tile_tensor = self._desc[rows.nbytes:]
             else:
                 self._desc[:rows.nbytes].copy_(torch.from_numpy(rows.view(np.uint8)).pin_memory(), non_blocking=True)
-        self.grads = grads
+        self.params, self.grads = params, grads
 
     @property
     def steps(self) -> torch.Tensor:

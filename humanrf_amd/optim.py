@@ -6,6 +6,7 @@ from __future__ import annotations
 from typing import Dict, Optional
 
 import torch
+from torch import Tensor
 
 from . import ops
 
@@ -42,7 +43,7 @@ class AdamW(torch.optim.Optimizer):
         return [p for group in self.param_groups for p in group["params"]]
 
     def _hyper(self):
-        """(lr, weight decay) of the call and the factors of each parameter."""
+        """(lr, weight decay) of the call and the factors of each group."""
         groups = self.param_groups
         first = groups[0]
         for g in groups:
@@ -57,7 +58,7 @@ class AdamW(torch.optim.Optimizer):
             scale = [float(g["lr"]) / lr if lr > 0.0 else 1.0 for g in groups]
         decay = max(float(g["weight_decay"]) for g in groups)
         decays = [float(g["weight_decay"]) / decay if decay > 0.0 else 1.0 for g in groups]
-        return lr, decay, [s for s, g in zip(scale, groups) for _ in g["params"]], [d for d, g in zip(decays, groups) for _ in g["params"]]
+        return lr, decay, scale, decays
 
     def _ensure_plan(self) -> ops.AdamWPlan:
         if self._plan is None:
@@ -75,22 +76,26 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         params = self._all()
         grads = [p.grad for p in params]
-        if all(g is None for g in grads):
+        present = [g for g in grads if g is not None]
+        if not present:
             return loss
         lr, decay, lr_scales, decay_scales = self._hyper()
         plan = self._ensure_plan()
-        key = ([(0 if g is None else g.data_ptr(), None if g is None else g.dtype) for g in grads], [p.data_ptr() for p in params],
-               lr_scales, decay_scales)
+        # What the descriptors depend on: storage that was replaced is checked again.
+        kind = lambda ts: (list(map(Tensor.data_ptr, ts)), list(map(Tensor.numel, ts)), [t.dtype for t in ts])  # noqa: E731
+        key = (kind(params), kind(present), [g is None for g in grads], lr_scales, decay_scales)
         if key != self._key:
-            for g in grads:
-                if g is not None and g.layout != torch.strided:
+            for g in present:
+                if g.layout != torch.strided:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
-            plan.params, plan.lr_scales, plan.decay_scales = [p.detach() for p in params], lr_scales, decay_scales
-            for p in plan.params:
-                ops._chk(p, "parameter")
-                if p.device != plan.device:
+            plan.lr_scales, plan.decay_scales = ([s for s, g in zip(scales, self.param_groups) for _ in g["params"]]
+                                                 for scales in (lr_scales, decay_scales))
+            if self._key is not None and key[0] == self._key[0]:
+                plan.set_grads(grads)
+            else:
+                if any(p.device != plan.device for p in params):
                     raise RuntimeError("AdamW: the parameters have moved to another device after the first step")
-            plan.set_grads(grads)
+                plan.set_tensors([p.detach() for p in params], grads)
             plan.grads = None            # (held by the parameters; a second reference here would keep dropped gradients alive)
             self._key = key
         group = self.param_groups[0]

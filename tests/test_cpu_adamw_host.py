@@ -1,0 +1,137 @@
+"""What humanrf_amd.optim.AdamW and ops.AdamWPlan put into the descriptors that the kernels follow, on the CPU: the library's calls are
+recorded instead of made, so that nothing is launched and a wrong address or length is seen without anybody following it."""
+import contextlib
+
+import numpy as np
+import pytest
+import torch
+
+
+class Recorder:
+    """Stands for the library: keeps what each call was given, the descriptors as they were at that moment."""
+
+    def __init__(self):
+        self.calls = []
+
+    def hrf_adamw_workspace_bytes(self):
+        return 64
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args, self.rows(args[0])))
+            return 0
+        return call
+
+    def rows(self, address):
+        from humanrf_amd import ops
+        import ctypes
+        raw = (ctypes.c_uint8 * (self.count * ops._ADAMW_TENSOR.itemsize)).from_address(address)
+        return np.frombuffer(bytes(raw), dtype=ops._ADAMW_TENSOR)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    from humanrf_amd import _lib, ops
+    lib, chk = Recorder(), ops._chk
+    monkeypatch.setattr(_lib, "lib", lambda: lib)
+    monkeypatch.setattr(ops, "_chk", lambda t, name, dtype=None, cuda=True: chk(t, name, dtype, False))
+    monkeypatch.setattr(ops, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "stream_of", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+    return lib
+
+
+def _stepped(host, tensors, **kw):
+    """An optimizer over parameters of these values that has taken one step."""
+    from humanrf_amd.optim import AdamW
+    params = [torch.nn.Parameter(t) for t in tensors]
+    host.count = len(params)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = AdamW(params, **kw)
+    opt.step()
+    return opt, params
+
+
+@pytest.mark.parametrize("length", [1000, 99_999, 100_001])
+def test_a_parameter_of_another_length_is_refused(host, length):
+    opt, (p, q) = _stepped(host, [torch.zeros(100_000), torch.zeros(7)])
+    assert host.calls[-1][2]["n"].tolist() == [100_000, 7]
+    n = len(host.calls)
+    p.grad = None
+    p.data = torch.zeros(length)
+    p.grad = torch.ones(length)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match=f"{length} values"):
+            opt.step()
+    assert len(host.calls) == n         # nothing was launched
+
+
+def test_a_parameter_cut_short_where_it_lies_is_refused(host):
+    opt, (p,) = _stepped(host, [torch.zeros(100)])
+    n, g = len(host.calls), p.grad
+    p.grad = None
+    p.data = p.data[:60]
+    p.grad = g[:60]                     # both at the addresses that they had
+    with pytest.raises(RuntimeError, match="60 values"):
+        opt.step()
+    assert len(host.calls) == n
+
+
+def test_storage_of_the_same_length_is_taken_over(host):
+    opt, (p, q) = _stepped(host, [torch.zeros(4, 10), torch.zeros(7)])
+    p.data = torch.full((5, 8), 2.0)
+    p.grad = torch.ones(5, 8, dtype=torch.float32)
+    opt.step()
+    rows = host.calls[-1][2]
+    assert rows["param"].tolist() == [p.data_ptr(), q.data_ptr()] and rows["grad"].tolist() == [p.grad.data_ptr(), q.grad.data_ptr()]
+    assert rows["n"].tolist() == [40, 7] and rows["kind"].tolist() == [0, 0]
+    p.grad = None
+    p.data = p.data.bfloat16()          # a type that the step knows: the descriptor says so
+    p.grad = torch.ones(5, 8, dtype=torch.bfloat16)
+    opt.step()
+    assert host.calls[-1][2]["kind"].tolist() == [2 | 2 << 2, 0] and host.calls[-1][2]["param"][0] == p.data_ptr()
+
+
+def test_replaced_storage_is_checked_as_the_first_was(host):
+    shared = torch.zeros(20)
+    for bad, said in ((torch.zeros(10, dtype=torch.float64), "must be float32"), (shared[:10], "share memory"),
+                      (torch.zeros(2, 5).t().contiguous().t().view(2, 5), "not contiguous")):
+        opt, (p, q) = _stepped(host, [torch.zeros(2, 5) if said == "not contiguous" else torch.zeros(10), shared[5:15]])
+        n = len(host.calls)
+        p.grad = None
+        p.data = bad
+        p.grad = torch.ones_like(bad)
+        with pytest.raises(RuntimeError, match=said):
+            opt.step()
+        assert len(host.calls) == n
+    p = torch.nn.Parameter(torch.zeros(10))
+    from humanrf_amd.optim import AdamW
+    host.count, p.grad = 1, torch.zeros(10)
+    opt = AdamW([p], copies={p: torch.zeros(10, dtype=torch.float16)})
+    opt.step()
+    p.grad = None
+    p.data = p.data.half()
+    p.grad = torch.zeros(10, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="copies of float32"):
+        opt.step()
+
+
+def test_plans_take_tensors_of_their_own_lengths_only(host):
+    from humanrf_amd import ops
+    host.count = 2
+    p, g = [torch.zeros(300), torch.zeros(5)], [torch.zeros(300), torch.zeros(5)]
+    plan = ops.AdamWPlan(p, g)
+    with pytest.raises(RuntimeError, match="as many parameters"):
+        plan.set_tensors(p[:1], g[:1])
+    with pytest.raises(RuntimeError, match="299 values"):
+        plan.set_tensors([p[0][:299], p[1]], [g[0][:299], g[1]])
+    with pytest.raises(RuntimeError, match="length and device"):
+        plan.set_tensors(p, [g[0][:299], g[1]])
+    assert plan.params is not None and [x.numel() for x in plan.params] == [300, 5]
+    q = [torch.ones(300), torch.ones(5)]
+    plan.set_tensors(q, [None, g[1]])
+    ops.adamw_multi(plan, 1e-2)
+    rows = host.calls[-1][2]
+    assert rows["param"].tolist() == [q[0].data_ptr(), q[1].data_ptr()] and rows["grad"].tolist() == [0, g[1].data_ptr()]
