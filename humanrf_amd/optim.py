@@ -81,8 +81,8 @@ class AdamW(torch.optim.Optimizer):
             return loss
         lr, decay, lr_scales, decay_scales = self._hyper()
         plan = self._ensure_plan()
-        # What the descriptors depend on: storage that was replaced is checked again.
-        kind = lambda ts: (list(map(Tensor.data_ptr, ts)), list(map(Tensor.numel, ts)), [t.dtype for t in ts])  # noqa: E731
+        # What the descriptors depend on: storage that was replaced, or a gradient that is now seen with other strides, is checked again.
+        kind = lambda ts: (list(map(Tensor.data_ptr, ts)), list(map(Tensor.numel, ts)), [t.dtype for t in ts], all(map(Tensor.is_contiguous, ts)))  # noqa: E731
         key = (kind(params), kind(present), [g is None for g in grads], lr_scales, decay_scales)
         if key != self._key:
             for g in present:

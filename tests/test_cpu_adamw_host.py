@@ -118,6 +118,23 @@ def test_replaced_storage_is_checked_as_the_first_was(host):
         opt.step()
 
 
+@pytest.mark.parametrize("other", [lambda b: b.view(16, 8).t(), lambda b: b[:1].expand(8, 16)], ids=["transposed", "broadcast"])
+def test_a_gradient_of_other_strides_at_the_same_address_is_refused(host, other):
+    opt, (p,) = _stepped(host, [torch.zeros(8, 16)])
+    buf = torch.zeros(128)
+    p.grad = buf.view(8, 16)
+    opt.step()
+    n = len(host.calls)
+    p.grad = other(buf)
+    assert p.grad.data_ptr() == buf.data_ptr() and p.grad.shape == (8, 16)
+    with pytest.raises(RuntimeError, match="not contiguous: gradient"):
+        opt.step(zero_grad=True)
+    assert len(host.calls) == n
+    p.grad = buf.view(8, 16)
+    opt.step()
+    assert len(host.calls) == n + 1
+
+
 def test_plans_take_tensors_of_their_own_lengths_only(host):
     from humanrf_amd import ops
     host.count = 2
