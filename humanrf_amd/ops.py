@@ -675,14 +675,11 @@ class AdamWPlan:
             if step:
                 self._ctl[_lib.ADAMW_CTL:] = int(step)
             self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
-        self.grads, self._desc = None, None
-        self._tiles = np.repeat(np.arange(len(params), dtype=np.int32), tiles)
+        self.grads, self._desc, self._desc_captured, self._kept = None, None, False, []
         self.set_grads([None] * len(params) if grads is None else grads)
-        del self._tiles
         # what the entry points take of the plan, as addresses: none of these buffers is ever replaced
         st = list(self.state.values())
         first, second, scales = (st[0], st[1], (None, None)) if self.state_bits == 32 else (st[0], st[2], (st[1], st[3]))
-        self._head = (ptr(self._desc), ptr(self._tile_tensor), self.num_tiles)
         self._body = (len(params), self.state_bits, ptr(first), ptr(second), ptr(scales[0]), ptr(scales[1]), ptr(self._ctl))
 
     def _take_state(self, state):
@@ -734,8 +731,16 @@ class AdamWPlan:
         self._point_at(params, grads)
 
     def set_grads(self, grads) -> None:
-        """Other gradient tensors (or None) for the next steps: the descriptors are written anew, on the current stream."""
+        """Other gradient tensors (or None) for the next steps: the descriptors are written anew, on the current stream. Replays of a
+        graph that captured adamw_multi or grad_norm_multi read the same descriptors, so these are their gradients too."""
         self._point_at(self.params, grads)
+
+    def _keep_captured(self, grads) -> None:
+        """The step that was just captured goes on reading its descriptors and these gradients: they stay, and the next change of addresses
+        is written into descriptors of its own."""
+        if not self._desc_captured:
+            self._kept.append((self._desc, self.params, list(grads)))
+            self._desc_captured = True
 
     def _point_at(self, params, grads) -> None:
         grads = list(grads)
@@ -760,10 +765,13 @@ class AdamWPlan:
         rows["kind"] = [_ADAMW_KINDS[p.dtype] | (_ADAMW_KINDS[g.dtype] << 2 if g is not None else 0) | (_ADAMW_KINDS[c.dtype] << 4 if c is not None else 0)
                         for p, g, c in zip(params, grads, self.copies)]
         rows["lr_scale"], rows["decay_scale"] = self.lr_scales, self.decay_scales
+        if self._desc_captured:
+            self._desc, self._desc_captured = None, False
         with _on_device(self.device):
             if self._desc is None:      # the descriptors, and behind them the tensor of each tile
-                self._desc = torch.from_numpy(np.concatenate([rows.view(np.uint8), self._tiles.view(np.uint8)])).to(self.device)
-                self._tile_tensor = self._desc[rows.nbytes:]
+                tiles = np.repeat(np.arange(len(rows), dtype=np.int32), -(-rows["n"] // self.TILE))
+                self._desc = torch.from_numpy(np.concatenate([rows.view(np.uint8), tiles.view(np.uint8)])).to(self.device)
+                self._head = (ptr(self._desc), ptr(self._desc) + rows.nbytes, self.num_tiles)
             else:
                 self._desc[:rows.nbytes].copy_(torch.from_numpy(rows.view(np.uint8)).pin_memory(), non_blocking=True)
         self.params, self.grads = params, grads

@@ -19,7 +19,8 @@ class AdamW(torch.optim.Optimizer):
 
     Gradients that stay in place from step to step (`zero_grad(set_to_none=False)`, or `step(zero_grad=True)`, which zeroes them in the
     same pass) cost nothing on the host; new ones are written into the descriptors first. A graph of the step is captured after one eager
-    step with the gradients in place. `step` advances the parameters' version counters, so that casts of them are renewed."""
+    step with the gradients in place; its replays step the tensors that it was captured with, whatever gradients later eager steps are given.
+    `step` advances the parameters' version counters, so that casts of them are renewed."""
 
     def __init__(self, params, lr=1e-2, betas=(0.9, 0.99), eps: float = 1e-15, weight_decay: float = 1e-2, state_bits: int = 32,
                  max_grad_norm: Optional[float] = None, seed: int = 0, copies: Optional[Dict[torch.Tensor, torch.Tensor]] = None):
@@ -102,6 +103,8 @@ class AdamW(torch.optim.Optimizer):
         norm = ops.grad_norm_multi(plan, grad_scale, scaler) if self.max_grad_norm is not None else None
         ops.adamw_multi(plan, lr, betas=group["betas"], eps=group["eps"], weight_decay=decay, norm=norm, max_norm=self.max_grad_norm,
                         grad_scale=grad_scale, flags=flags, scaler=scaler, zero_grad=zero_grad)
+        if torch.cuda.is_current_stream_capturing():
+            plan._keep_captured(grads)
         torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
         return loss
 

@@ -152,3 +152,26 @@ def test_plans_take_tensors_of_their_own_lengths_only(host):
     ops.adamw_multi(plan, 1e-2)
     rows = host.calls[-1][2]
     assert rows["param"].tolist() == [q[0].data_ptr(), q[1].data_ptr()] and rows["grad"].tolist() == [0, g[1].data_ptr()]
+
+
+def test_a_captured_step_keeps_its_descriptors(host, monkeypatch):
+    """A graph holds the address of the descriptors. Eager steps with other gradients write theirs elsewhere, so that replays neither step with
+    gradients that they were not captured with nor follow addresses of tensors that are gone."""
+    import gc
+    import weakref
+    opt, (p, q) = _stepped(host, [torch.zeros(3000), torch.zeros(7)], max_grad_norm=1.0)
+    held = weakref.ref(p.grad)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step(zero_grad=True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    captured, rows = host.calls[-1][1][:2], host.calls[-1][2]
+    for _ in range(3):
+        p.grad, q.grad = torch.ones(3000), None
+        opt.step()
+        _, args, now = host.calls[-1]
+        assert args[0] != captured[0] and now["grad"].tolist() == [p.grad.data_ptr(), 0]
+        assert args[1] == args[0] + now.nbytes
+    gc.collect()
+    assert held() is not None and np.array_equal(host.rows(captured[0]), rows)
+    # eager steps alone rewrite the descriptors that they have
+    assert len({args[0] for _, args, _ in host.calls[-3:]}) == 1

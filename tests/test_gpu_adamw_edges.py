@@ -1,0 +1,52 @@
+"""The AdamW step's entry points in calls that other tests do not make: captured steps next to eager ones of other gradients, loss scales without
+a norm, values whose squares leave fp32, plans of empty tensors, optimizers that are copied. Tolerances: U = 2^-24 is half a step of fp32."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+LR = 1e-2
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _params(sizes, seed):
+    g = _gen(seed)
+    return [torch.nn.Parameter(torch.randn(n, generator=g, device="cuda")) for n in sizes]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_step_what_was_captured(bits):
+    """A captured step, eager steps with gradient tensors of their own between its replays: the same bits as a twin that is given each
+    gradient in turn."""
+    from humanrf_amd.optim import AdamW
+    sizes = (5000, 33)
+    ps, qs = _params(sizes, 0), _params(sizes, 0)
+    opt, twin = AdamW(ps, max_grad_norm=1.0, state_bits=bits), AdamW(qs, max_grad_norm=1.0, state_bits=bits)
+    static = [torch.randn(n, generator=_gen(n), device="cuda") for n in sizes]
+    given = lambda o, params, grads: ([setattr(p, "grad", g) for p, g in zip(params, grads)], o.step())  # noqa: E731
+    given(opt, ps, static)
+    given(twin, qs, static)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step()
+    for k in range(4):
+        graph.replay()
+        given(twin, qs, [g.clone() for g in static])
+        other = [torch.randn(n, generator=_gen(100 + k), device="cuda") for n in sizes]
+        given(opt, ps, other)
+        given(twin, qs, other)
+        for p in ps:
+            p.grad = None
+        del other
+        torch.full((50_000,), 1e9, device="cuda")           # what was freed is used by somebody else
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    assert opt._plan.steps.tolist() == twin._plan.steps.tolist() == [9, 9]
