@@ -465,6 +465,7 @@ extern "C" int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* t
                   std::isfinite(weight_decay) && weight_decay >= 0.0 && aw_scaled(grad_scale), "bad hyper-parameters");
     HRF_CHECK_ARG(std::isfinite(eps) && (float)eps >= 1.17549435e-38f, "eps has to be a positive normal fp32 number");
     HRF_CHECK_ARG(!(max_norm > 0.0) || norm, "clipping needs the norm of the gradients");
+    HRF_CHECK_ARG(!scaler || norm || flags, "a loss scale needs the norm of the gradients or flags to see that they are finite");
     if (num_tiles == 0) return 0;
     HRF_CHECK_ARG(tensors && tile_tensor && exp_avg && second && ctl, "NULL argument");
     HRF_CHECK_ARG(state_bits == 32 || (exp_avg_scale && second_scale), "8-bit states need their scales");

@@ -807,7 +807,8 @@ def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weig
     """torch.optim.AdamW step of every tensor of the plan that has a gradient, in one launch (hrf_adamw_multi, include/hrf.h).
     lr: a number, or an fp32 tensor of one value on the device (a schedule inside a captured graph). norm: what grad_norm_multi gave for
     these gradients; a norm that is not finite skips the step, and with max_norm the gradients are scaled down to that norm. flags:
-    int32 (>= 1,), the step is skipped when flags[0] != 0. scaler: ops.grad_scaler, gradients are unscaled and its scale is updated."""
+    int32 (>= 1,), the step is skipped when flags[0] != 0. scaler: ops.grad_scaler, gradients are unscaled and its scale is updated, as
+    torch.amp.GradScaler does; where neither norm nor flags say whether the gradients are finite, their norm is taken first."""
     lr_dev = None
     if isinstance(lr, torch.Tensor):
         _chk(lr, "lr", torch.float32)
@@ -822,6 +823,8 @@ def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weig
             raise RuntimeError("adamw_multi: lr, norm, flags and scaler hold a value")
     if max_norm is not None and (norm is None or not float(max_norm) > 0.0):
         raise RuntimeError("adamw_multi: max_norm is a positive number and needs the norm of the gradients")
+    if scaler is not None and norm is None and flags is None:
+        norm = grad_norm_multi(plan, grad_scale, scaler)
     with _on_device(plan.device), _span("adamw", plan.numel):
         check(_lib.lib().hrf_adamw_multi(*plan._head, *plan._body, float(lr), ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
                                          float(weight_decay), float(grad_scale), 0.0 if max_norm is None else float(max_norm), ptr(norm),

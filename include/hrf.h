@@ -541,7 +541,8 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
  *   counts of the tensors that have a gradient.
  * lr: host value, or DEVICE fp32 lr_dev (may be NULL). Gradients are divided by grad_scale (times scaler->scale when a scaler is given)
  *   and, with max_norm > 0, multiplied by min(1, max_norm / (*norm + 1e-6)). The step is skipped (steps and values stay) when
- *   flags[0] != 0 or *norm (either may be NULL) is not finite; with a scaler its scale is then backed off, and grown as GradScaler does.
+ *   flags[0] != 0 or *norm (either may be NULL; not both with a scaler) is not finite; with a scaler its scale is then backed off, and grown as
+ *   GradScaler does.
  * zero_grad != 0: the gradients are zeroed in the same pass. eps must be a positive normal fp32 number. */
 #define HRF_ADAMW_TICKETS 32
 #define HRF_ADAMW_CTL (32 + 32 * (1 + HRF_ADAMW_TICKETS)) /* counters of finished workgroups, each on a cache line of its own */

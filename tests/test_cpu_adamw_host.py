@@ -175,3 +175,25 @@ def test_a_captured_step_keeps_its_descriptors(host, monkeypatch):
     assert held() is not None and np.array_equal(host.rows(captured[0]), rows)
     # eager steps alone rewrite the descriptors that they have
     assert len({args[0] for _, args, _ in host.calls[-3:]}) == 1
+
+
+def test_a_loss_scale_alone_has_the_norm_taken(host):
+    """Without a norm and without flags nothing would see an overflowed gradient, and the scale would only grow."""
+    from humanrf_amd import ops
+    opt, (p,) = _stepped(host, [torch.zeros(50)])
+    scaler, flags = ops.grad_scaler("cpu"), torch.zeros(1, dtype=torch.int32)
+    del host.calls[:]
+    opt.step(scaler=scaler, grad_scale=2.0)
+    (norm, norm_args, _), (step, args, _) = host.calls
+    assert norm == "hrf_grad_norm_multi" and norm_args[3:5] == (2.0, scaler.data_ptr()) and step == "hrf_adamw_multi"
+    assert args[-6] == norm_args[6] and args[-4] == scaler.data_ptr()
+    del host.calls[:]
+    opt.step(scaler=scaler, flags=flags)
+    assert [c[0] for c in host.calls] == ["hrf_adamw_multi"] and host.calls[0][1][-6:-3] == (None, flags.data_ptr(), scaler.data_ptr())
+
+
+def test_the_entry_refuses_a_loss_scale_alone():
+    from humanrf_amd import _lib
+    lib, fake = _lib.lib(), 1 << 20      # an address that is never followed
+    args = [fake, fake, 1, 1, 32, fake, fake, None, None, fake, 1e-2, None, 0.9, 0.99, 1e-15, 0.0, 1.0, 0.0, None, None, fake, 0, 0, None]
+    assert lib.hrf_adamw_multi(*args) != 0 and b"loss scale" in lib.hrf_last_error()

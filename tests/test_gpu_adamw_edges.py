@@ -50,3 +50,37 @@ def test_replays_step_what_was_captured(bits):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, qs))
     assert opt._plan.steps.tolist() == twin._plan.steps.tolist() == [9, 9]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("through", ["optimizer", "plan"])
+def test_a_loss_scale_alone_skips_what_overflowed(bits, through):
+    from humanrf_amd import ops
+    from humanrf_amd.optim import AdamW
+    p, = _params((3000,), 1)
+    scaler = ops.grad_scaler("cuda", init_scale=1024.0, growth_interval=2)
+    if through == "optimizer":
+        opt = AdamW([p], state_bits=bits)
+        step = lambda: opt.step(scaler=scaler)  # noqa: E731
+        plan = lambda: opt._plan  # noqa: E731
+        p.grad = torch.randn(3000, device="cuda") * 1024.0
+    else:
+        grad = torch.randn(3000, device="cuda") * 1024.0
+        made = ops.AdamWPlan([p.detach()], [grad], state_bits=bits)
+        step = lambda: ops.adamw_multi(made, LR, scaler=scaler)  # noqa: E731
+        plan = lambda: made  # noqa: E731
+        p.grad = grad
+    step()
+    assert plan().steps.tolist() == [1] and ops.grad_scaler_state(scaler)["growth_tracker"] == 1
+    old, states = p.detach().clone(), {k: v.clone() for k, v in plan().state.items()}
+    for bad in (float("inf"), float("nan")):
+        kept = p.grad[2999].clone()
+        p.grad[2999] = bad
+        step()
+        p.grad[2999] = kept
+        assert torch.equal(p, old) and all(torch.equal(v.float(), plan().state[k].float()) for k, v in states.items())
+    assert plan().steps.tolist() == [1] and plan().skipped.item() == 2
+    assert ops.grad_scaler_state(scaler)["scale"] == 256.0 and ops.grad_scaler_state(scaler)["growth_tracker"] == 0
+    step()
+    step()
+    assert plan().steps.tolist() == [3] and ops.grad_scaler_state(scaler)["scale"] == 512.0
