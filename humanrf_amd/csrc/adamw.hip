@@ -122,21 +122,21 @@ __device__ __forceinline__ double aw_pow(double b, int32_t t)   // b^t by squari
     return r;
 }
 
-// Square root and quotient from the hardware's approximations (1 ulp) and one correction by the remainder, which an fma gives exactly:
-// at most a few thousandths of an ulp over correct rounding, in 6 and 5 instructions where the library's take 18 and 11. The range is
-// what the step needs and no more. Root: 0 stays 0; what is positive counts as 2^-126 at least, and as the largest finite number at
-// most (a second moment beyond fp32 saturates). Quotient: a normal denominator.
+// Square root and quotient from the hardware's approximations (1 ulp) and one step of Newton's method, whose remainder an fma gives
+// exactly: at most a few thousandths of an ulp over correct rounding, in 7 and 6 instructions where the library's take 18 and 11.
+// Root: what is positive counts as 2^-126 at least; 0, inf and NaN are their own roots: a second moment beyond fp32 has no finite
+// root, and the step that is divided by it is 0. Quotient: a denominator that is normal, inf or NaN.
 __device__ __forceinline__ float aw_sqrt(float x)
 {
-    const float c = __builtin_amdgcn_fmed3f(x, 1.17549435e-38f, 3.402823466e38f);
+    const float c = fmaxf(x, 1.17549435e-38f);
     const float y = __builtin_amdgcn_rsqf(c), s = c * y;
     const float r = fmaf(fmaf(-s, s, c), 0.5f * y, s);
-    return x > 0.0f ? r : 0.0f;
+    return __builtin_amdgcn_classf(x, 0x180) ? r : x;       // positive, normal (0x100) or not (0x080)
 }
 __device__ __forceinline__ float aw_divide(float a, float b)
 {
     const float y = __builtin_amdgcn_rcpf(b), q = a * y;
-    return fmaf(fmaf(-q, b, a), y, q);
+    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-q, b, a), y, q), b, a);
 }
 
 // fp8 conversions of exactly representable values

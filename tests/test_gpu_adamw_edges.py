@@ -84,3 +84,45 @@ def test_a_loss_scale_alone_skips_what_overflowed(bits, through):
     step()
     step()
     assert plan().steps.tolist() == [3] and ops.grad_scaler_state(scaler)["scale"] == 512.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [1e22, 1e25, 1e30, 3e38])
+def test_gradients_whose_squares_leave_fp32(bits, size):
+    """The second moment is inf, as in torch's own fp32 step: the first moment over it is 0, and the value decays and does nothing else. With
+    8-bit states the scale of the block's roots is inf. In the next step the block's other codes, 0 times inf, are NaN, and so are their values;
+    the code of the inf itself is the largest, 448 times inf is inf, and its value is divided by that again."""
+    from humanrf_amd import ops
+    p = torch.randn(600, generator=_gen(2), device="cuda")
+    g = torch.randn(600, generator=_gen(3), device="cuda")
+    g[300] = -size
+    p0, want = p.clone(), torch.nn.Parameter(p.clone())
+    want.grad = g.clone()
+    torch.optim.AdamW([want], lr=LR, betas=(0.9, 0.99), eps=1e-15, weight_decay=0.1, foreach=False).step()
+    plan = ops.AdamWPlan([p], [g], state_bits=bits)
+    ops.adamw_multi(plan, LR, eps=1e-15, weight_decay=0.1)
+    tol = 8 * U * p0.double().abs() + 40 * U * LR
+    assert bool(((p.double() - want.detach().double()).abs() <= tol).all())
+    assert float(p[300]) == float(p0[300] * torch.tensor(1.0 - LR * 0.1))
+    if bits == 32:
+        assert math.isinf(float(plan.state["exp_avg_sq"][300])) and int(torch.isfinite(plan.state["exp_avg_sq"]).sum()) == plan.numel - 1
+        assert abs(float(plan.state["exp_avg"][300]) + 0.1 * size) <= 4 * U * 0.1 * size
+    else:
+        assert torch.isfinite(plan.state["exp_avg_root_scale"]).tolist() == [True, False, True]
+    g[300] = 0.0
+    ops.adamw_multi(plan, LR, eps=1e-15)
+    gone = ~torch.isfinite(p)
+    assert int(gone.sum()) == (0 if bits == 32 else 255) and (bits == 32 or (bool(gone[256:300].all()) and bool(gone[301:512].all())))
+
+
+def test_a_root_that_is_not_finite_is_seen():
+    """A second moment that is NaN, under a first moment that is finite: the root's scale, and the value, are NaN."""
+    from humanrf_amd import ops
+    for bits in (32, 8):
+        p, g = torch.ones(600, device="cuda"), torch.ones(600, device="cuda")
+        plan = ops.AdamWPlan([p], [g], state_bits=bits)
+        plan.state["exp_avg_sq" if bits == 32 else "exp_avg_root_scale"][300 if bits == 32 else 1] = float("nan")
+        ops.adamw_multi(plan, LR)
+        gone = torch.isnan(p)
+        assert int(gone.sum()) == (1 if bits == 32 else 256) and bool(gone[300])
+        assert bits == 32 or torch.isnan(plan.state["exp_avg_root_scale"]).tolist() == [False, True, False]
