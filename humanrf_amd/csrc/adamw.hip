@@ -123,14 +123,15 @@ __device__ __forceinline__ double aw_pow(double b, int32_t t)   // b^t by squari
 }
 
 // Square root and quotient from the hardware's approximations (1 ulp) and one step of Newton's method, whose remainder an fma gives
-// exactly: at most a few thousandths of an ulp over correct rounding, in 7 and 6 instructions where the library's take 18 and 11.
-// Root: what is positive counts as 2^-126 at least; 0, inf and NaN are their own roots: a second moment beyond fp32 has no finite
-// root, and the step that is divided by it is 0. Quotient: a denominator that is normal, inf or NaN.
+// exactly: at most a few thousandths of an ulp over correct rounding, in 11 and 6 instructions where the library's take 18 and 11.
+// Root: below 2^-100 the value is taken times 2^64 (the approximation flushes what is not normal); 0, inf and NaN are their own roots: a
+// second moment beyond fp32 has no finite root, and the step that is divided by it is 0. Quotient: a denominator that is normal, inf or NaN.
 __device__ __forceinline__ float aw_sqrt(float x)
 {
-    const float c = fmaxf(x, 1.17549435e-38f);
+    const bool tiny = x < 0x1p-100f;
+    const float c = ldexpf(x, tiny ? 64 : 0);
     const float y = __builtin_amdgcn_rsqf(c), s = c * y;
-    const float r = fmaf(fmaf(-s, s, c), 0.5f * y, s);
+    const float r = ldexpf(fmaf(fmaf(-s, s, c), 0.5f * y, s), tiny ? -32 : 0);
     return __builtin_amdgcn_classf(x, 0x180) ? r : x;       // positive, normal (0x100) or not (0x080)
 }
 __device__ __forceinline__ float aw_divide(float a, float b)

@@ -126,3 +126,27 @@ def test_a_root_that_is_not_finite_is_seen():
         gone = torch.isnan(p)
         assert int(gone.sum()) == (1 if bits == 32 else 256) and bool(gone[300])
         assert bits == 32 or torch.isnan(plan.state["exp_avg_root_scale"]).tolist() == [False, True, False]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_second_moments_below_the_normal_numbers(bits):
+    """Gradients of 1e-19 to 1e-21 under an eps that does not hide them: the root is that of the moment as fp32 holds it, v <= 2^-126 being a
+    multiple of 2^-149. The update from that v is bounded as everywhere else: 24 U, and v itself by 8 U v + 2^-149."""
+    from humanrf_amd import ops
+    for size in (1e-19, 3e-20, 1e-20, 1e-21):
+        g = torch.full((512,), size, device="cuda") * (1.0 + torch.arange(512, device="cuda") % 7 / 8)
+        p = torch.zeros(512, device="cuda")
+        plan = ops.AdamWPlan([p], [g], state_bits=bits)
+        ops.adamw_multi(plan, LR, betas=(0.9, 0.99), eps=1e-36)
+        v = g.double().square() * 0.01
+        held = torch.round(v * 2.0 ** 149) * 2.0 ** -149
+        if bits == 32:
+            held = plan.state["exp_avg_sq"][:512].double()
+            assert bool(((held - v).abs() <= 8 * U * v + 2.0 ** -149).all())
+        root = held.sqrt()
+        want = -LR / 0.1 * (0.1 * g.double()) / (root / 0.1)
+        spread = 0.0 if bits == 32 else 2.0 ** -149 / held       # (half a multiple up or down in v, halved by the root, and as much again)
+        assert bool(((p.double() - want).abs() <= (24 * U + spread) * want.abs()).all()), size
+        if bits == 8:
+            top = root.view(2, 256).amax(1)
+            assert bool(((plan.state["exp_avg_root_scale"].double() * 448 - top).abs() <= (8 * U + 2.0 ** -149 / held.min()) * top).all())
