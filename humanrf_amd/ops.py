@@ -874,7 +874,7 @@ def quantize_int8(x: torch.Tensor):
 class Int8Weight:
     """A layer's weights for linear_int8, laid out once: from codes int8 (channels, inner), one fp32 scale per channel and an fp32 bias per
     channel or None. `packed` holds a copy of the codes in the order in which the product reads them (hrf_int8_pack, include/hrf.h); scale
-    and bias are kept, not copied. `from_float` rounds a weight matrix (channels, inner)."""
+    and bias are kept, not copied. `from_float` rounds a weight matrix (channels, inner) and copies its bias."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
         if codes.dim() != 2 or codes.dtype != torch.int8:
@@ -901,7 +901,8 @@ class Int8Weight:
         if weight.dim() != 2:
             raise RuntimeError("Int8Weight: the weight must be a matrix (channels, inner)")
         codes, scale = quantize_int8(weight.detach())
-        return cls(codes, scale, None if bias is None else bias.detach().float().contiguous())
+        # (a copy: the layer that the bias comes from may be trained on, and a handle's may be loaded over)
+        return cls(codes, scale, None if bias is None else bias.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format))
 
     @classmethod
     def from_packed(cls, packed: torch.Tensor, out_features: int, in_features: int, scale: torch.Tensor,

@@ -1,0 +1,53 @@
+"""What humanrf_amd.int8's modules hold and hand to the product, on the CPU: the library's calls are replaced, nothing is launched."""
+import contextlib
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """-> the handles that products were called with."""
+    from humanrf_amd import _lib, ops
+    chk, handles = ops._chk, []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    def quantize(x):
+        scale = x.abs().amax(1) / 127.0
+        return torch.round(x / scale[:, None]).to(torch.int8), scale
+
+    def linear(x, weight, relu=False, out_dtype=None):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("linear_int8: no gradient flows")
+        handles.append(weight)
+        return x.new_zeros(*x.shape[:-1], weight.out_features)
+    monkeypatch.setattr(_lib, "lib", Library)
+    monkeypatch.setattr(ops, "_chk", lambda t, name, dtype=None, cuda=True: chk(t, name, dtype, False))
+    monkeypatch.setattr(ops, "_rows_of", lambda t, name: t)
+    monkeypatch.setattr(ops, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "stream_of", lambda index: 0)
+    monkeypatch.setattr(ops, "quantize_int8", quantize)
+    monkeypatch.setattr(ops, "linear_int8", linear)
+    return handles
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_served_layer_has_a_bias_of_its_own(host, dtype):
+    from humanrf_amd.int8 import Int8Linear, Int8MLP
+    net = torch.nn.Linear(20, 10).to(dtype)
+    served = Int8Linear.from_linear(net)
+    want = net.bias.detach().float().clone()
+    with torch.no_grad():
+        net.bias += 1.0                                     # training goes on
+    assert torch.equal(served.bias, want) and served.bias.dtype == torch.float32
+    trained = net.bias.detach().clone()
+    other = Int8Linear.from_linear(torch.nn.Linear(20, 10))
+    served.load_state_dict(other.state_dict())              # another checkpoint is loaded into the served layer
+    assert torch.equal(net.bias, trained) and torch.equal(served.bias, other.bias)
+    strided = torch.arange(20.0)[::2]
+    assert Int8Linear(torch.ones(10, 4), strided).bias.tolist() == strided.tolist()
+    mlp = Int8MLP.from_sequential(torch.nn.Sequential(net, torch.nn.ReLU()))
+    assert mlp[0].bias.data_ptr() != net.bias.data_ptr()
