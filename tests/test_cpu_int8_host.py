@@ -51,3 +51,31 @@ def test_a_served_layer_has_a_bias_of_its_own(host, dtype):
     assert Int8Linear(torch.ones(10, 4), strided).bias.tolist() == strided.tolist()
     mlp = Int8MLP.from_sequential(torch.nn.Sequential(net, torch.nn.ReLU()))
     assert mlp[0].bias.data_ptr() != net.bias.data_ptr()
+
+
+def test_buffers_that_are_replaced_are_the_ones_multiplied_with(host):
+    from humanrf_amd.int8 import Int8Linear
+    make = lambda: Int8Linear.from_linear(torch.nn.Linear(20, 10))  # noqa: E731
+    served, x = make(), torch.zeros(3, 20)
+
+    def used():
+        served(x)
+        h = host[-1]
+        assert h.packed is served.packed and h.scale is served.scale and h.bias is served.bias
+        return h
+    used()
+    used()
+    assert host[-1] is host[-2]
+    other = make()
+    served.load_state_dict(other.state_dict(), assign=True)
+    assert torch.equal(used().scale, other.scale)
+    for name in ("packed", "scale", "bias"):
+        setattr(served, name, getattr(served, name).clone())
+        used()
+    served.bias = None
+    assert used().bias is None
+    served.bias = other.bias
+    third = make()
+    torch.func.functional_call(served, dict(third.named_buffers()), (x,))
+    assert host[-1].packed is third.packed and host[-1].scale is third.scale and host[-1].bias is third.bias
+    used()
