@@ -36,13 +36,13 @@ class Int8Linear(torch.nn.Module):
         self._handle = None
         return out
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor, out_dtype=None) -> torch.Tensor:
+        """No gradients flow: an x that needs one is refused outside torch.no_grad()."""
         held, now = self._handle, self._buffers
         # (buffers are replaced by load_state_dict(assign=True), torch.func.functional_call, or a plain assignment)
         if held is None or held.packed is not now["packed"] or held.scale is not now["scale"] or held.bias is not now["bias"]:
             held = self._handle = ops.Int8Weight.from_packed(now["packed"], self.out_features, self.in_features, now["scale"], now["bias"])
-        return ops.linear_int8(x.detach(), held, relu=self.relu, out_dtype=out_dtype)
+        return ops.linear_int8(x, held, relu=self.relu, out_dtype=out_dtype)
 
     def extra_repr(self) -> str:
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, relu={self.relu}"

@@ -79,3 +79,15 @@ def test_buffers_that_are_replaced_are_the_ones_multiplied_with(host):
     torch.func.functional_call(served, dict(third.named_buffers()), (x,))
     assert host[-1].packed is third.packed and host[-1].scale is third.scale and host[-1].bias is third.bias
     used()
+
+
+def test_inputs_that_need_a_gradient_are_refused(host):
+    from humanrf_amd.int8 import Int8Linear, Int8MLP
+    net = torch.nn.Sequential(torch.nn.Linear(20, 10), torch.nn.ReLU(), torch.nn.Linear(10, 4))
+    x = torch.zeros(3, 20, requires_grad=True)
+    for served in (Int8Linear.from_linear(net[0]), Int8MLP.from_sequential(net)):
+        with pytest.raises(RuntimeError, match="no gradient flows"):
+            served(x)
+        with torch.no_grad():
+            assert not served(x).requires_grad
+        assert not served(x.detach()).requires_grad
