@@ -10,7 +10,8 @@ from . import ops
 
 
 class Int8Linear(torch.nn.Module):
-    """y = act(x W^T + b), W in 8 bits: buffers `packed` (codes), `scale` (out), `bias` (out) or None."""
+    """y = act(x W^T + b), W in 8 bits: buffers `packed` (codes), `scale` (out), `bias` (out) or None. The state dict also names the layer's
+    widths, since rows of different lengths may be padded to the same one."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor = None, relu: bool = False):
         super().__init__()
@@ -24,6 +25,22 @@ class Int8Linear(torch.nn.Module):
     @classmethod
     def from_linear(cls, linear: torch.nn.Linear, relu: bool = False) -> "Int8Linear":
         return cls(linear.weight, linear.bias, relu)
+
+    def get_extra_state(self) -> torch.Tensor:
+        return torch.tensor([self.in_features, self.out_features])
+
+    def set_extra_state(self, state) -> None:
+        pass
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "_extra_state"
+        widths = state_dict.get(key)
+        if widths is not None and widths.tolist() != [self.in_features, self.out_features]:
+            error_msgs.append(f"Int8Linear {prefix[:-1]}: weights (in, out) = {tuple(widths.tolist())} for a layer of {(self.in_features, self.out_features)}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if widths is None and key in missing_keys:
+            missing_keys.remove(key)        # written before the widths were
 
     def _apply(self, fn, recurse=True):
         kept = (self.scale, self.bias)

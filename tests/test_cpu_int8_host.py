@@ -92,3 +92,26 @@ def test_inputs_that_need_a_gradient_are_refused(host):
         with torch.no_grad():
             assert not served(x).requires_grad
         assert not served(x.detach()).requires_grad
+
+
+def test_a_checkpoint_of_another_width_is_refused(host):
+    """Rows of 100 and of 120 codes are both padded to 128."""
+    from humanrf_amd.int8 import Int8Linear, Int8MLP
+    make = lambda k: Int8Linear.from_linear(torch.nn.Linear(k, 10))  # noqa: E731
+    served, same, wider = make(100), make(100), make(120)
+    assert served.packed.shape == wider.packed.shape
+    before = served.bias.clone()
+    for assign in (False, True):
+        with pytest.raises(RuntimeError, match=r"\(120, 10\).*\(100, 10\)"):
+            served.load_state_dict(wider.state_dict(), assign=assign)
+        assert torch.equal(served.bias, before)
+    served.load_state_dict(same.state_dict())
+    assert torch.equal(served.bias, same.bias)
+    old = {k: v for k, v in make(100).state_dict().items() if k in ("packed", "scale", "bias")}       # without the widths
+    served.load_state_dict(old)
+    assert torch.equal(served.bias, old["bias"])
+    with pytest.raises(RuntimeError, match="Missing"):
+        served.load_state_dict({k: v for k, v in old.items() if k != "scale"})
+    net = torch.nn.Sequential(torch.nn.Linear(100, 10), torch.nn.ReLU(), torch.nn.Linear(10, 4))
+    a, b = Int8MLP.from_sequential(net), Int8MLP.from_sequential(torch.nn.Sequential(torch.nn.Linear(100, 10), torch.nn.Linear(10, 4)))
+    assert list(a.load_state_dict(b.state_dict())) == [[], []]
