@@ -46,6 +46,14 @@ __device__ __forceinline__ float i8_factor(uint32_t top, float& scale)
 // Four values -> four codes in one word. |x| * factor is below 127.0001 (and 0 * NaN converts to 0), so that no clamp is needed.
 __device__ __forceinline__ uint32_t i8_code(float x, float factor, bool finite) { return finite ? (uint32_t)(int)rintf(x * factor) & 0xffu : 0u; }
 
+// A launch has fewer than 2^32 threads along an axis: past 2^22 workgroups they are counted along the second one too.
+#define I8_GRID_X (1 << 22)
+static dim3 i8_grid(int64_t blocks)
+{
+    return blocks <= I8_GRID_X ? dim3((unsigned)blocks) : dim3(I8_GRID_X, (unsigned)((blocks + I8_GRID_X - 1) / I8_GRID_X));
+}
+__device__ __forceinline__ int64_t i8_block() { return (int64_t)blockIdx.y * I8_GRID_X + blockIdx.x; }
+
 // Where code k of a row goes. Packed: see above. Otherwise rows of `ld` codes.
 template <bool kPacked>
 __device__ __forceinline__ int64_t i8_at(int64_t row, int k, int64_t ld)
@@ -62,7 +70,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
     __shared__ uint32_t s_max[4];
     constexpr int n = I8Piece<K>::n, kRows = 256 / kGroup;
     const int lane = threadIdx.x % kGroup;
-    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kGroup;
+    const int64_t row = i8_block() * kRows + threadIdx.x / kGroup;
     const bool here = row < rows;
     const typename I8Type<K>::T* const from = x + (here ? row : rows - 1) * ldx;
     I8Piece<K> v[kPieces];
@@ -111,12 +119,14 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>:
 
 // Rows too long for the registers: read twice, the second time from the cache. Also codes at any address.
 template <int K, bool kPacked>
-__global__ __launch_bounds__(256) void k_quantize_rows_long(const typename I8Type<K>::T* __restrict__ x, int cols, int64_t ldx,
+__global__ __launch_bounds__(256) void k_quantize_rows_long(const typename I8Type<K>::T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                             int8_t* __restrict__ q, int ldq, float* __restrict__ scale)
 {
     __shared__ uint32_t s_max[4];
     constexpr int n = I8Piece<K>::n;
-    const typename I8Type<K>::T* const from = x + (int64_t)blockIdx.x * ldx;
+    const int64_t row = i8_block();
+    if (row >= rows) return;
+    const typename I8Type<K>::T* const from = x + row * ldx;
     auto get = [&](int k0, I8Piece<K>& v) {
         if (k0 + n <= cols) i8_get<K>(v, from + k0);
         else {
@@ -139,11 +149,11 @@ __global__ __launch_bounds__(256) void k_quantize_rows_long(const typename I8Typ
     float sc;
     const float factor = i8_factor(top, sc);
     const bool finite = top < 0x7f800000u;
-    if (threadIdx.x == 0) scale[blockIdx.x] = sc;
+    if (threadIdx.x == 0) scale[row] = sc;
     for (int k0 = threadIdx.x * n; k0 < ldq; k0 += 256 * n) {
         I8Piece<K> v;
         get(k0, v);
-        int8_t* const to = q + i8_at<kPacked>(blockIdx.x, k0, ldq);
+        int8_t* const to = q + i8_at<kPacked>(row, k0, ldq);
         int8_t code[n];
 #pragma unroll
         for (int k = 0; k < n; ++k) code[k] = (int8_t)i8_code(I8Type<K>::up(v.v[k]), factor, finite);
@@ -157,10 +167,12 @@ __global__ __launch_bounds__(256) void k_quantize_rows_long(const typename I8Typ
 }
 
 // Rows of codes -> rows padded with zeros to ldq, a multiple of 16 bytes.
-__global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, int cols, int64_t ldx, int8_t* __restrict__ q, int ldq)
+__global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ q, int ldq)
 {
-    x += (int64_t)blockIdx.x * ldx;
-    q += (int64_t)blockIdx.x * ldq;
+    const int64_t row = i8_block();
+    if (row >= rows) return;
+    x += row * ldx;
+    q += row * ldq;
     for (int k0 = threadIdx.x * 16; k0 < ldq; k0 += 4096) {
         i8_v4 v = {0, 0, 0, 0};
         if (k0 + 16 <= cols) __builtin_memcpy(&v, x + k0, 16);
@@ -174,7 +186,7 @@ __global__ __launch_bounds__(256) void k_pad_rows(const int8_t* __restrict__ x, 
 __global__ __launch_bounds__(256) void k_pack_rows(const int8_t* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                    int8_t* __restrict__ packed, int64_t padded, int64_t pieces)
 {
-    const int64_t piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t piece = i8_block() * 256 + threadIdx.x;
     if (piece >= pieces) return;
     const int64_t block = piece >> 6, runs = padded >> 6, row = block / runs * 16 + (piece & 15);
     const int k0 = (int)(block % runs) * 64 + ((int)(piece >> 4) & 3) * 16;
@@ -666,10 +678,10 @@ static void i8_quantize(const void* xv, int64_t rows, int64_t cols, int64_t ldx,
     constexpr int n = I8Piece<K>::n;
     const bool pieces = (((uintptr_t)q | (uintptr_t)ldq) & 7u) == 0;
 #define I8_ROWS(G, P)                                                                                                                  \
-    hipLaunchKernelGGL((k_quantize_rows<K, kPacked, G, P>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))), dim3(256), 0, stream, x, rows, \
+    hipLaunchKernelGGL((k_quantize_rows<K, kPacked, G, P>), i8_grid((rows + 256 / G - 1) / (256 / G)), dim3(256), 0, stream, x, rows, \
                        (int)cols, ldx, q, ldq, scale)
     if (!pieces || ldq > 256 * 8 * n)
-        hipLaunchKernelGGL((k_quantize_rows_long<K, kPacked>), dim3((unsigned)rows), dim3(256), 0, stream, x, (int)cols, ldx, q, (int)ldq, scale);
+        hipLaunchKernelGGL((k_quantize_rows_long<K, kPacked>), i8_grid(rows), dim3(256), 0, stream, x, rows, (int)cols, ldx, q, (int)ldq, scale);
     else if (ldq <= 16 * n) I8_ROWS(16, 1);
     else if (ldq <= 64 * n) I8_ROWS(64, 1);
     else if (ldq <= 64 * 4 * n) I8_ROWS(64, 4);
@@ -690,7 +702,7 @@ static void i8_rows(const void* x, int x_type, int64_t rows, int64_t cols, int64
 static void i8_pack(const int8_t* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* packed, hipStream_t stream)
 {
     const int64_t padded = i8_padded(cols), pieces = (rows + 15) / 16 * padded;
-    hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, x, rows, (int)cols, ldx, packed, padded, pieces);
+    hipLaunchKernelGGL(k_pack_rows, i8_grid((pieces + 255) / 256), dim3(256), 0, stream, x, rows, (int)cols, ldx, packed, padded, pieces);
 }
 
 // Rows of up to 256 values, where rounding them first (a launch, codes written and read again) costs more than reading x once for every 64
@@ -735,20 +747,25 @@ static void i8_few(const I8Args& A, hipStream_t stream)
 }
 
 template <int K, int TM, int TN, int WN, int R>
-static void i8_tiles(const I8Args& A, hipStream_t stream)
+static int i8_tiles(const I8Args& A, hipStream_t stream)
 {
     const int64_t tiles = (int64_t)((A.rows + 64 * TM - 1) / (64 * TM)) * ((A.cols + 32 * TN * WN - 1) / (32 * TN * WN));
+    if (tiles * 128 * WN >= (int64_t)1 << 32) {
+        hrf_set_error("hrf_linear_int8: too many tiles");
+        return 1;
+    }
     hipLaunchKernelGGL((k_linear_i8<K, TM, TN, WN, R>), dim3((unsigned)tiles), dim3(128 * WN), 0, stream, A);
+    return 0;
 }
 
 #define I8_FEW 64       // rows up to which the product of few tokens runs, on packed codes
 
 template <int K>
-static void i8_linear(const I8Args& A, hipStream_t stream)
+static int i8_linear(const I8Args& A, hipStream_t stream)
 {
-    if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return; }
-    if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return; }
-    if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return; }
+    if (A.rows <= 16) { i8_few<K, 1, 1>(A, stream); return 0; }
+    if (A.rows <= 32) { i8_few<K, 2, 2>(A, stream); return 0; }
+    if (A.rows <= I8_FEW) { i8_few<K, 4, 2>(A, stream); return 0; }
     // Rounds of the card times what a round of that size takes against one of 128 x 128: larger tiles read each operand less often, smaller ones
     // fill the card when there is little, and a round that only a few tiles need takes as long as a full one (264 tiles of 128 on 256
     // CUs: two). Captured calls in us, rounding included, with 64 / 128 / 128 x 192 / 256:
@@ -759,14 +776,14 @@ static void i8_linear(const I8Args& A, hipStream_t stream)
     // of the smaller tiles: 6465 x 1799 x 214 27 / 21 / 24 / 23.
     auto rounds = [&](int m, int n) { return (((int64_t)A.rows + m - 1) / m * (((int64_t)A.cols + n - 1) / n) + 255) / 256; };
     const int64_t c64 = 9 * rounds(64, 64), c128 = 20 * rounds(128, 128), c192 = 25 * rounds(128, 192), c256 = 60 * rounds(256, 256);
-    if (A.inner >= 512 && c256 < std::min(std::min(c64, c128), c192)) i8_tiles<K, 4, 2, 4, 1>(A, stream);
-    else if (A.inner >= 512 && c192 < std::min(c64, c128)) i8_tiles<K, 2, 3, 2, 1>(A, stream);
-    else if (c128 < c64) i8_tiles<K, 2, 2, 2, 1>(A, stream);
-    else i8_tiles<K, 1, 1, 2, 2>(A, stream);
+    if (A.inner >= 512 && c256 < std::min(std::min(c64, c128), c192)) return i8_tiles<K, 4, 2, 4, 1>(A, stream);
+    if (A.inner >= 512 && c192 < std::min(c64, c128)) return i8_tiles<K, 2, 3, 2, 1>(A, stream);
+    if (c128 < c64) return i8_tiles<K, 2, 2, 2, 1>(A, stream);
+    return i8_tiles<K, 1, 1, 2, 2>(A, stream);
 }
 
 template <int K>
-static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const float* x_scale, int inner, void* workspace, hipStream_t stream)
+static int i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const float* x_scale, int inner, void* workspace, hipStream_t stream)
 {
     if (i8_is_short(A.rows, A.cols, A.inner)) {
         I8Short B;
@@ -775,7 +792,7 @@ static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const 
         else if (x_type == I8_F16) i8_short<I8_F16, K>(A, B, stream);
         else if (x_type == I8_BF16) i8_short<I8_BF16, K>(A, B, stream);
         else i8_short<I8_INT8, K>(A, B, stream);
-        return;
+        return 0;
     }
     if (i8_is_one(A.rows, A.inner, x_type)) {
         I8Short B;
@@ -783,7 +800,7 @@ static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const 
         if (x_type == I8_F32) i8_one<I8_F32, K>(A, B, stream);
         else if (x_type == I8_F16) i8_one<I8_F16, K>(A, B, stream);
         else i8_one<I8_BF16, K>(A, B, stream);
-        return;
+        return 0;
     }
     float* const scale = (float*)((int8_t*)workspace + ((int64_t)A.rows + 15) / 16 * 16 * A.inner);
     A.x = (const int8_t*)workspace;
@@ -799,9 +816,14 @@ static void i8_product(I8Args& A, const void* x, int x_type, int64_t ldx, const 
         A.x = (const int8_t*)x;         // rows that lie as the tiles read them
         A.ldx = ldx;
     } else {
-        hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)A.rows), dim3(256), 0, stream, (const int8_t*)x, inner, ldx, (int8_t*)workspace, A.inner);
+        hipLaunchKernelGGL(k_pad_rows, i8_grid(A.rows), dim3(256), 0, stream, (const int8_t*)x, (int64_t)A.rows, inner, ldx, (int8_t*)workspace, A.inner);
     }
-    i8_linear<K>(A, stream);
+    const hipError_t rounded = hipGetLastError();       // (no product of codes that nobody wrote)
+    if (rounded != hipSuccess) {
+        hrf_set_error("hrf_linear_int8: launch failed: %s", hipGetErrorString(rounded));
+        return 2;
+    }
+    return i8_linear<K>(A, stream);
 }
 
 static bool i8_inner_ok(int64_t inner) { return inner >= 1 && inner <= HRF_INT8_MAX_INNER; }
@@ -836,7 +858,6 @@ extern "C" int hrf_int8_pack(const int8_t* q, int64_t rows, int64_t cols, int64_
     HRF_CHECK_ARG(q && packed, "NULL argument");
     HRF_CHECK_ARG(ldq >= cols || rows == 1, "a row stride is shorter than the row");
     HRF_CHECK_ARG(((uintptr_t)packed & 15u) == 0, "the packed codes must begin at a multiple of 16 bytes");
-    HRF_CHECK_ARG(hrf_int8_packed_bytes(rows, cols) < (int64_t)16 * 256 * 2147483647, "too many codes");
     i8_pack(q, rows, cols, ldq, packed, (hipStream_t)stream);
     HRF_CHECK_LAUNCH();
     return 0;
@@ -859,9 +880,11 @@ extern "C" int hrf_linear_int8(const void* x, int x_type, int64_t ldx, const flo
     I8Args A;
     A.x = nullptr; A.ldx = 0; A.w = w; A.sx = nullptr; A.sw = w_scale; A.bias = bias; A.y = y; A.ldy = ldy;
     A.rows = (int)rows; A.cols = (int)cols; A.inner = i8_padded(inner); A.relu = relu;
-    if (y_type == I8_F32) i8_product<I8_F32>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
-    else if (y_type == I8_F16) i8_product<I8_F16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
-    else i8_product<I8_BF16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    int rc;
+    if (y_type == I8_F32) rc = i8_product<I8_F32>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    else if (y_type == I8_F16) rc = i8_product<I8_F16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    else rc = i8_product<I8_BF16>(A, x, x_type, ldx, x_scale, (int)inner, workspace, (hipStream_t)stream);
+    if (rc != 0) return rc;
     HRF_CHECK_LAUNCH();
     return 0;
 }

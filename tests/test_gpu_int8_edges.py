@@ -1,0 +1,57 @@
+"""The 8-bit product's entry points in calls that other tests do not make: more rows than one axis of a launch counts, codes of several axes,
+scales at the ends of fp32, modules whose buffers are replaced. Tolerances: U = 2^-24 is half a step of fp32."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _codes(m, k, seed):
+    return torch.randint(-128, 128, (m, k), generator=_gen(seed), device="cuda", dtype=torch.int8)
+
+
+# ------------------------------------------------------------------------------------------------ past 2^32 threads
+@pytest.mark.parametrize("m,k,ld", [(2 ** 24 + 37, 3, 3), (2 ** 28 + 5, 3, 8)], ids=["a workgroup a row", "16 rows a workgroup"])
+def test_rounding_more_rows_than_an_axis_counts(m, k, ld):
+    from humanrf_amd import _lib
+    from humanrf_amd._lib import check, ptr, stream_ptr
+    x = torch.randn(m, k, generator=_gen(0), device="cuda", dtype=F16)
+    q, s = torch.full((m, ld), 99, dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda")
+    check(_lib.lib().hrf_quantize_rows_int8(ptr(x), 1, m, k, k, ptr(q), ld, ptr(s), stream_ptr()))
+    for at in range(0, m, 2 ** 26):         # everything, in pieces
+        part = slice(at, min(m, at + 2 ** 26))
+        top = x[part].float().abs().amax(1).clamp(min=2.0 ** -119)
+        assert torch.equal(s[part], top * (1.0 / 127.0))
+        assert bool(((q[part, :k].float() * s[part, None] - x[part].float()).abs() <= s[part, None] * (0.5 + 127 * 6 * U)).all())
+        assert int(q[part, k:].ne(0).sum()) == 0
+
+
+def test_products_of_more_rows_than_an_axis_counts():
+    """Codes of 130 a row are padded into the workspace, a workgroup a row."""
+    from humanrf_amd import ops
+    m, k, n = 2 ** 24 + 37, 130, 200
+    x, w = _codes(m, k, 1), _codes(n, k, 2)
+    sx, sw = torch.rand(m, generator=_gen(3), device="cuda") + 0.5, torch.rand(n, generator=_gen(4), device="cuda") + 0.5
+    y = ops.linear_int8(x, ops.Int8Weight(w, sw), x_scale=sx, out_dtype=BF16)
+    for rows in (slice(0, 300), slice(2 ** 22 - 100, 2 ** 22 + 100), slice(2 ** 24 - 100, m)):
+        v = (x[rows].double() @ w.double().t()) * sx[rows].double()[:, None] * sw.double()
+        assert bool(((y[rows].double() - v).abs() <= (2.0 ** -8 + 4 * U) * v.abs()).all())
+
+
+def test_packing_more_rows_than_an_axis_counts():
+    """One code a row, 64 bytes a row packed: more than 2^30 pieces of 16 bytes, which is where the second axis begins."""
+    from humanrf_amd import ops
+    n = 2 ** 28 + 16
+    w = _codes(n, 1, 5)
+    p = ops.Int8Weight(w, torch.ones(n, device="cuda")).packed.view(n // 16, 64, 16)
+    assert torch.equal(p[:, :16, 0].reshape(n, 1), w)       # row t of a block: the 16 bytes at 16 t
+    for at in range(0, n // 16, 2 ** 22):
+        part = p[at:at + 2 ** 22]
+        assert int(part[:, :, 1:].ne(0).sum()) == 0 and int(part[:, 16:].ne(0).sum()) == 0
