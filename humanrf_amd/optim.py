@@ -84,11 +84,13 @@ class AdamW(torch.optim.Optimizer):
         plan = self._ensure_plan()
         # What the descriptors depend on: storage that was replaced, or a gradient that is now seen with other strides, is checked again.
         kind = lambda ts: (list(map(Tensor.data_ptr, ts)), list(map(Tensor.numel, ts)), [t.dtype for t in ts], all(map(Tensor.is_contiguous, ts)))  # noqa: E731
-        key = (kind(params), kind(present), [g is None for g in grads], lr_scales, decay_scales)
+        try:
+            key = (kind(params), kind(present), [g is None for g in grads], lr_scales, decay_scales)
+        except RuntimeError:        # (a sparse tensor has no address)
+            if all(g.layout == torch.strided for g in present):
+                raise
+            raise RuntimeError("AdamW: sparse gradients are not supported") from None
         if key != self._key:
-            for g in present:
-                if g.layout != torch.strided:
-                    raise RuntimeError("AdamW: sparse gradients are not supported")
             plan.lr_scales, plan.decay_scales = ([s for s, g in zip(scales, self.param_groups) for _ in g["params"]]
                                                  for scales in (lr_scales, decay_scales))
             if self._key is not None and key[0] == self._key[0]:

@@ -197,3 +197,13 @@ def test_the_entry_refuses_a_loss_scale_alone():
     lib, fake = _lib.lib(), 1 << 20      # an address that is never followed
     args = [fake, fake, 1, 1, 32, fake, fake, None, None, fake, 1e-2, None, 0.9, 0.99, 1e-15, 0.0, 1.0, 0.0, None, None, fake, 0, 0, None]
     assert lib.hrf_adamw_multi(*args) != 0 and b"loss scale" in lib.hrf_last_error()
+
+
+def test_sparse_gradients_are_refused_by_name(host):
+    opt, (p, q) = _stepped(host, [torch.zeros(4, 4), torch.zeros(7)])
+    n = len(host.calls)
+    q.grad = None
+    p.grad = torch.eye(4).to_sparse()
+    with pytest.raises(RuntimeError, match="sparse gradients"):
+        opt.step()
+    assert len(host.calls) == n
