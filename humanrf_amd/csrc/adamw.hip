@@ -16,6 +16,7 @@
 // ones, whose 88 vector instructions an element keep the vector unit busy three quarters of that time; the norm of 240 M fp32 gradients
 // 161 us (6.0 TB/s).
 #include "hrf_common.h"
+#include <algorithm>
 #include <cmath>
 
 #define AW_TILE 2048    // elements of one tensor that a workgroup of 256 works on at a time: two times four per thread
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(256) void k_adamw(const hrf_adamw_tensor* __restric
 {
     __shared__ int s_last;
     const int tile_end = min(num_tiles, (int)(blockIdx.x + 1) * per);
-    int which = tile_tensor[blockIdx.x * per];
+    int which = num_tiles > 0 ? tile_tensor[blockIdx.x * per] : 0;
     double inv = C.inv_grad_scale, lr = C.lr;
     if (C.scaler) inv /= (double)C.scaler->scale;
     if (C.lr_dev) lr = (double)*C.lr_dev;
@@ -467,9 +468,9 @@ extern "C" int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* t
     HRF_CHECK_ARG(std::isfinite(eps) && (float)eps >= 1.17549435e-38f, "eps has to be a positive normal fp32 number");
     HRF_CHECK_ARG(!(max_norm > 0.0) || norm, "clipping needs the norm of the gradients");
     HRF_CHECK_ARG(!scaler || norm || flags, "a loss scale needs the norm of the gradients or flags to see that they are finite");
-    if (num_tiles == 0) return 0;
-    HRF_CHECK_ARG(tensors && tile_tensor && exp_avg && second && ctl, "NULL argument");
-    HRF_CHECK_ARG(state_bits == 32 || (exp_avg_scale && second_scale), "8-bit states need their scales");
+    if (num_tiles == 0 && (count == 0 || !tensors)) return 0;
+    HRF_CHECK_ARG(tensors && ctl && (num_tiles == 0 || (tile_tensor && exp_avg && second)), "NULL argument");
+    HRF_CHECK_ARG(state_bits == 32 || num_tiles == 0 || (exp_avg_scale && second_scale), "8-bit states need their scales");
     HRF_CHECK_ARG((((uintptr_t)exp_avg | (uintptr_t)second) & 15u) == 0, "states must begin at multiples of 16 bytes");
     AwConst C;
     C.lr = lr; C.beta1 = beta1; C.beta2 = beta2;
@@ -481,7 +482,7 @@ extern "C" int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* t
     // workgroup computes once (the bias corrections, in fp64) counts: four neighbouring tiles each, where that leaves eight workgroups
     // for every CU. 240 M parameters 698 us against 749 with one tile each, 39 M 134 against 146.
     const int per = state_bits == 8 && num_tiles >= 4 * 2048 ? 4 : 1;
-    const unsigned blocks = (unsigned)((num_tiles + per - 1) / per);
+    const unsigned blocks = (unsigned)std::max(1, (num_tiles + per - 1) / per);    // (tensors without a value have a step count)
     if (state_bits == 32)
         hipLaunchKernelGGL(k_adamw<32>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, tensors, tile_tensor, num_tiles, count, exp_avg,
                            second, nullptr, nullptr, ctl, per, C);

@@ -538,7 +538,7 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
  *   state_bits 8:  exp_avg, second = e4m3 (OCP fn) codes of m and of sqrt(v), exp_avg_scale / second_scale = fp32, one per block. Codes
  *                  are rounded up or down at random, without bias, by a hash of (seed, step, position): the same call gives the same bits.
  * ctl: DEVICE int32[HRF_ADAMW_CTL + count] = { steps skipped, internal ..., steps[count] }, zero at first. The launch advances the step
- *   counts of the tensors that have a gradient.
+ *   counts of the tensors that have a gradient, empty ones too (num_tiles 0: nothing else; with tensors NULL, nothing at all).
  * lr: host value, or DEVICE fp32 lr_dev (may be NULL). Gradients are divided by grad_scale (times scaler->scale when a scaler is given)
  *   and, with max_norm > 0, multiplied by min(1, max_norm / (*norm + 1e-6)). The step is skipped (steps and values stay) when
  *   flags[0] != 0 or *norm (either may be NULL; not both with a scaler) is not finite; with a scaler its scale is then backed off, and grown as

@@ -150,3 +150,22 @@ def test_second_moments_below_the_normal_numbers(bits):
         if bits == 8:
             top = root.view(2, 256).amax(1)
             assert bool(((plan.state["exp_avg_root_scale"].double() * 448 - top).abs() <= (8 * U + 2.0 ** -149 / held.min()) * top).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_empty_tensors_alone_have_step_counts(bits):
+    """As an empty tensor among others has: steps, skipped steps and the loss scale go on."""
+    from humanrf_amd import ops
+    empty = lambda: torch.zeros(0, device="cuda")  # noqa: E731
+    plan = ops.AdamWPlan([empty(), empty()], [empty(), None], state_bits=bits)
+    ops.adamw_multi(plan, LR)
+    ops.adamw_multi(plan, LR, norm=ops.grad_norm_multi(plan), max_norm=1.0)
+    assert plan.steps.tolist() == [2, 0] and plan.skipped.item() == 0
+    scaler = ops.grad_scaler("cuda", init_scale=64.0, growth_interval=1)
+    ops.adamw_multi(plan, LR, flags=torch.ones(1, dtype=torch.int32, device="cuda"), scaler=scaler)
+    assert plan.steps.tolist() == [2, 0] and plan.skipped.item() == 1 and ops.grad_scaler_state(scaler)["scale"] == 32.0
+    ops.adamw_multi(plan, LR, scaler=scaler, zero_grad=True)
+    assert plan.steps.tolist() == [3, 0] and ops.grad_scaler_state(scaler)["scale"] == 64.0
+    mixed = ops.AdamWPlan([empty(), torch.zeros(5, device="cuda")], [empty(), torch.ones(5, device="cuda")], state_bits=bits)
+    ops.adamw_multi(mixed, LR)
+    assert mixed.steps.tolist() == [1, 1]
