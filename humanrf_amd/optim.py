@@ -122,26 +122,32 @@ class AdamW(torch.optim.Optimizer):
                 out[name] = buf[at:at + n].view(self._plan.params[k].shape)
         return out
 
+    def _entries(self) -> dict:
+        if self._plan is None:
+            return {}
+        steps = self._plan.steps.cpu()
+        return {k: {"step": steps[k].float(), **{name: v.clone() for name, v in self._views(k).items()}} for k in range(len(self._plan.params))}
+
     def state_dict(self):
         """torch.optim.AdamW's layout: per parameter "step", "exp_avg", "exp_avg_sq" (with 8 bits "exp_avg", "exp_avg_root" and their
         scales instead); a checkpoint with 32-bit states loads into either."""
         sd = super().state_dict()
-        if self._plan is not None:
-            steps = self._plan.steps.cpu()
-            sd["state"] = {k: {"step": steps[k].float(), **{name: v.clone() for name, v in self._views(k).items()}}
-                           for k in range(len(self._plan.params))}
+        sd["state"] = self._entries()
         return sd
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         self._hyper()
+        self._take_entries(state_dict["state"])
+
+    def _take_entries(self, entries) -> None:
         plan = self._ensure_plan()
         for buf in plan.state.values():
             buf.view(torch.uint8).zero_()
         plan.steps.zero_()
         for k in range(len(plan.params)):
-            entry = state_dict["state"].get(k)
+            entry = entries.get(k)
             if not entry:
                 continue
             for name, view in self._views(k).items():
@@ -156,6 +162,22 @@ class AdamW(torch.optim.Optimizer):
                     view.copy_(value)
             plan.steps[k] = int(entry["step"])
         self._key = None
+
+    # copies and pickles: the plan, whose addresses are this object's own, is built again over the copy's parameters
+    def __getstate__(self):
+        own = {name: getattr(self, name) for name in ("state_bits", "max_grad_norm", "seed", "_copies")}
+        return {**super().__getstate__(), **own, "entries": self._entries()}
+
+    def __setstate__(self, state) -> None:
+        state = dict(state)
+        copied = "entries" in state         # (torch's load_state_dict comes here too, with groups alone)
+        entries = state.pop("entries", None)
+        super().__setstate__(state)
+        if copied:
+            self._plan, self._key = None, None
+        if entries:
+            with torch.no_grad():
+                self._take_entries(entries)
 
 
 __all__ = ["AdamW"]

@@ -207,3 +207,49 @@ def test_sparse_gradients_are_refused_by_name(host):
     with pytest.raises(RuntimeError, match="sparse gradients"):
         opt.step()
     assert len(host.calls) == n
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_and_pickles_of_an_optimizer(host, how, bits):
+    """A copy steps its own parameters, from the states and step counts that it was made with."""
+    import copy
+    import io
+    net = torch.nn.Linear(20, 5)
+    from humanrf_amd.optim import AdamW
+    copies = {net.weight: torch.zeros(5, 20, dtype=torch.float16)}
+    opt = AdamW(net.parameters(), lr=3e-3, state_bits=bits, max_grad_norm=2.0, seed=7, copies=copies)
+    host.count = 2
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+
+    def again(pair):
+        if how == "deepcopy":
+            return copy.deepcopy(pair)
+        file = io.BytesIO()
+        torch.save(pair, file)
+        return torch.load(io.BytesIO(file.getvalue()), weights_only=False)
+    fresh_net, fresh = again((net, opt))                 # before the first step
+    assert fresh._plan is None and fresh.max_grad_norm == 2.0 and fresh.state_bits == bits
+    opt.step()
+    for k, buf in enumerate(opt._plan.state.values()):
+        buf.view(torch.uint8)[:5] = k + 1
+    opt._plan.steps[:] = torch.tensor([3, 4], dtype=torch.int32)
+    other_net, other = again((net, opt))
+    for p in list(other_net.parameters()) + list(fresh_net.parameters()):
+        p.grad = torch.ones_like(p)
+    for made, made_net in ((other, other_net), (fresh, fresh_net)):
+        made.step()
+        rows = host.calls[-1][2]
+        assert rows["param"].tolist() == [p.data_ptr() for p in made_net.parameters()]
+        assert rows["copy"].tolist()[0] == made._copies[made_net.weight].data_ptr() != copies[net.weight].data_ptr()
+        assert host.calls[-1][1][10] == 3e-3 and host.calls[-1][1][21] == 7
+    assert other._plan.steps.tolist() == [3, 4] and fresh._plan.steps.tolist() == [0, 0]
+    for name, buf in opt._plan.state.items():
+        assert torch.equal(buf.view(torch.uint8), other._plan.state[name].view(torch.uint8))
+        assert buf.data_ptr() != other._plan.state[name].data_ptr()
+    # the original goes on, and so does loading
+    opt.step()
+    assert host.calls[-1][2]["param"].tolist() == [p.data_ptr() for p in net.parameters()]
+    other.load_state_dict(opt.state_dict())
+    assert other._plan.steps.tolist() == opt._plan.steps.tolist()

@@ -169,3 +169,24 @@ def test_empty_tensors_alone_have_step_counts(bits):
     mixed = ops.AdamWPlan([empty(), torch.zeros(5, device="cuda")], [empty(), torch.ones(5, device="cuda")], state_bits=bits)
     ops.adamw_multi(mixed, LR)
     assert mixed.steps.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_of_the_optimizer_goes_on_as_the_original(bits):
+    import copy
+    from humanrf_amd.optim import AdamW
+    ps = _params((3000, 7), 5)
+    opt = AdamW(ps, state_bits=bits, max_grad_norm=1.0, seed=11)
+
+    def step(o, params, seed):
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=_gen(seed), device="cuda")
+        o.step()
+    step(opt, ps, 0)
+    qs, other = copy.deepcopy((ps, opt))
+    for k in range(1, 4):
+        step(opt, ps, k)
+        step(other, qs, k)
+    assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(ps, qs))
+    assert all(torch.equal(v.float(), other._plan.state[n].float()) for n, v in opt._plan.state.items())
+    assert other._plan.steps.tolist() == [4, 4]
