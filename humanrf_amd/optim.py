@@ -43,9 +43,9 @@ class AdamW(torch.optim.Optimizer):
     def _all(self):
         return [p for group in self.param_groups for p in group["params"]]
 
-    def _hyper(self):
+    def _hyper(self, groups=None):
         """(lr, weight decay) of the call and the factors of each group."""
-        groups = self.param_groups
+        groups = self.param_groups if groups is None else groups
         first = groups[0]
         for g in groups:
             if tuple(g["betas"]) != tuple(first["betas"]) or g["eps"] != first["eps"]:
@@ -137,9 +137,27 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        self._hyper()
+        """All of a checkpoint, or none of it: one that does not fit is refused before anything is changed."""
+        groups = state_dict["param_groups"]
+        self._hyper(groups)
+        self._check_entries(state_dict["state"])
+        super().load_state_dict({"state": {}, "param_groups": groups})
         self._take_entries(state_dict["state"])
+
+    def _check_entries(self, entries) -> None:
+        plan = self._ensure_plan()
+        for k in range(len(plan.params)):
+            entry = entries.get(k)
+            if not entry:
+                continue
+            for name, view in self._views(k).items():
+                if name not in entry:
+                    raise RuntimeError(f"AdamW: the checkpoint has no {name} for parameter {k}: was it written with states in other bits?")
+                value = entry[name]
+                if value.shape != view.shape or (view.dtype == torch.float8_e4m3fn) != (value.dtype == torch.float8_e4m3fn):
+                    raise RuntimeError(f"AdamW: {name} of parameter {k} has another shape or type in the checkpoint")
+            if int(entry["step"]) < 0:
+                raise RuntimeError(f"AdamW: negative step count of parameter {k} in the checkpoint")
 
     def _take_entries(self, entries) -> None:
         plan = self._ensure_plan()
@@ -151,11 +169,7 @@ class AdamW(torch.optim.Optimizer):
             if not entry:
                 continue
             for name, view in self._views(k).items():
-                if name not in entry:
-                    raise RuntimeError(f"AdamW: the checkpoint has no {name} for parameter {k}: was it written with states in other bits?")
                 value = entry[name]
-                if value.shape != view.shape or (view.dtype == torch.float8_e4m3fn) != (value.dtype == torch.float8_e4m3fn):
-                    raise RuntimeError(f"AdamW: {name} of parameter {k} has another shape or type in the checkpoint")
                 if view.dtype == torch.float8_e4m3fn:
                     view.view(torch.uint8).copy_(value.view(torch.uint8))
                 else:

@@ -253,3 +253,51 @@ def test_copies_and_pickles_of_an_optimizer(host, how, bits):
     assert host.calls[-1][2]["param"].tolist() == [p.data_ptr() for p in net.parameters()]
     other.load_state_dict(opt.state_dict())
     assert other._plan.steps.tolist() == opt._plan.steps.tolist()
+
+
+def _checkpoint(opt):
+    import copy
+    return copy.deepcopy(opt.state_dict())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_that_does_not_fit_changes_nothing(host, bits):
+    opt, params = _stepped(host, [torch.zeros(6, 5), torch.zeros(7)], lr=3e-3, state_bits=bits)
+    for buf in opt._plan.state.values():
+        buf.view(torch.uint8).fill_(3)
+    opt._plan.steps[:] = 5
+    before = {name: buf.clone() for name, buf in opt._plan.state.items()}
+
+    def spoil(change):
+        sd = _checkpoint(opt)
+        for entry in sd["state"].values():
+            for v in entry.values():
+                v.view(torch.uint8).fill_(9) if v.dim() else None
+        sd["param_groups"][0]["lr"] = 1.0
+        change(sd)
+        return sd
+    cases = [(lambda sd: sd["state"][1].pop("exp_avg"), "has no exp_avg for parameter 1"),
+             (lambda sd: sd["state"][1].update(exp_avg=sd["state"][1]["exp_avg"][:6]), "parameter 1 has another shape"),
+             (lambda sd: sd["state"][0].update(exp_avg=sd["state"][0]["exp_avg"].to(torch.float32 if bits == 8 else torch.float8_e4m3fn)), "another shape or type"),
+             (lambda sd: sd["state"][1].update(step=torch.tensor(-1.0)), "negative step")]
+    for change, said in cases:
+        with pytest.raises((RuntimeError, ValueError), match=said):
+            opt.load_state_dict(spoil(change))
+        assert all(torch.equal(buf.view(torch.uint8), before[name].view(torch.uint8)) for name, buf in opt._plan.state.items())
+        assert opt._plan.steps.tolist() == [5, 5] and opt.param_groups[0]["lr"] == 3e-3
+    opt.load_state_dict(spoil(lambda sd: None))
+    assert opt.param_groups[0]["lr"] == 1.0
+    assert int(opt._plan.state["exp_avg"].view(torch.uint8)[0]) == 9
+
+
+def test_groups_that_do_not_fit_change_nothing(host):
+    opt, params = _stepped(host, [torch.zeros(6), torch.zeros(7)])
+    from humanrf_amd.optim import AdamW
+    opt = AdamW([{"params": params[:1]}, {"params": params[1:]}], lr=3e-3)
+    opt.step()
+    opt._plan.state["exp_avg"].fill_(2.0)
+    sd = _checkpoint(opt)
+    sd["param_groups"][1]["eps"] = 1e-3
+    with pytest.raises(ValueError, match="betas and eps"):
+        opt.load_state_dict(sd)
+    assert opt.param_groups[1]["eps"] == 1e-15 and float(opt._plan.state["exp_avg"][0]) == 2.0
