@@ -139,6 +139,9 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """All of a checkpoint, or none of it: one that does not fit is refused before anything is changed."""
         groups = state_dict["param_groups"]
+        for g in groups:
+            if g.get("amsgrad") or g.get("maximize") or (g.get("decoupled_weight_decay") is False and g["weight_decay"] != 0):
+                raise ValueError("AdamW: the checkpoint's optimizer has amsgrad, maximize or coupled weight decay")
         self._hyper(groups)
         self._check_entries(state_dict["state"])
         super().load_state_dict({"state": {}, "param_groups": groups})

@@ -279,7 +279,10 @@ def test_a_checkpoint_that_does_not_fit_changes_nothing(host, bits):
     cases = [(lambda sd: sd["state"][1].pop("exp_avg"), "has no exp_avg for parameter 1"),
              (lambda sd: sd["state"][1].update(exp_avg=sd["state"][1]["exp_avg"][:6]), "parameter 1 has another shape"),
              (lambda sd: sd["state"][0].update(exp_avg=sd["state"][0]["exp_avg"].to(torch.float32 if bits == 8 else torch.float8_e4m3fn)), "another shape or type"),
-             (lambda sd: sd["state"][1].update(step=torch.tensor(-1.0)), "negative step")]
+             (lambda sd: sd["state"][1].update(step=torch.tensor(-1.0)), "negative step"),
+             (lambda sd: sd["param_groups"][0].update(amsgrad=True), "amsgrad"),
+             (lambda sd: sd["param_groups"][0].update(maximize=True), "maximize"),
+             (lambda sd: sd["param_groups"][0].update(decoupled_weight_decay=False), "coupled")]
     for change, said in cases:
         with pytest.raises((RuntimeError, ValueError), match=said):
             opt.load_state_dict(spoil(change))
@@ -301,3 +304,7 @@ def test_groups_that_do_not_fit_change_nothing(host):
     with pytest.raises(ValueError, match="betas and eps"):
         opt.load_state_dict(sd)
     assert opt.param_groups[1]["eps"] == 1e-15 and float(opt._plan.state["exp_avg"][0]) == 2.0
+    torch_s = torch.optim.AdamW(params, amsgrad=True)
+    torch_s.step()
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW(params).load_state_dict(torch_s.state_dict())
