@@ -50,6 +50,9 @@ class AdamW(torch.optim.Optimizer):
         for g in groups:
             if tuple(g["betas"]) != tuple(first["betas"]) or g["eps"] != first["eps"]:
                 raise ValueError("AdamW: betas and eps are the same in all parameter groups")
+            # (a factor of the largest would be stepped with, whatever its sign)
+            if not 0.0 <= float(g["weight_decay"]) < float("inf") or not (isinstance(g["lr"], torch.Tensor) or 0.0 <= float(g["lr"]) < float("inf")):
+                raise ValueError(f"AdamW: lr and weight_decay are finite and not negative, got {g['lr']} and {g['weight_decay']}")
         if any(isinstance(g["lr"], torch.Tensor) for g in groups):
             if any(g["lr"] is not first["lr"] for g in groups):
                 raise ValueError("AdamW: an lr that is a tensor is the same tensor in all parameter groups")

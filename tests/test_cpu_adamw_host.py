@@ -308,3 +308,24 @@ def test_groups_that_do_not_fit_change_nothing(host):
     torch_s.step()
     with pytest.raises(ValueError, match="amsgrad"):
         AdamW(params).load_state_dict(torch_s.state_dict())
+
+
+@pytest.mark.parametrize("bad", [dict(lr=-1e-3), dict(weight_decay=-0.1), dict(lr=float("nan")), dict(lr=float("inf")), dict(weight_decay=float("nan"))],
+                         ids=str)
+def test_every_group_s_lr_and_decay_are_looked_at(host, bad):
+    """One negative next to a positive one became a negative factor, and the group climbed; max() of a NaN is whichever comes first."""
+    from humanrf_amd.optim import AdamW
+    make = lambda **kw: [{"params": [torch.nn.Parameter(torch.zeros(4))]}, {"params": [torch.nn.Parameter(torch.zeros(4))], **kw}]  # noqa: E731
+    with pytest.raises(ValueError, match="finite and not negative"):
+        AdamW(make(**bad))
+    groups = make()
+    host.count = 2
+    opt = AdamW(groups)
+    for g in opt.param_groups:
+        g["params"][0].grad = torch.ones(4)
+    opt.step()
+    n = len(host.calls)
+    opt.param_groups[1].update(bad)         # as a schedule would
+    with pytest.raises(ValueError, match="finite and not negative"):
+        opt.step()
+    assert len(host.calls) == n
