@@ -775,6 +775,9 @@ class AdamWPlan:
             else:
                 self._desc[:rows.nbytes].copy_(torch.from_numpy(rows.view(np.uint8)).pin_memory(), non_blocking=True)
         self.params, self.grads = params, grads
+        # what a step writes, for autograd and for casts that are renewed by version; views of one tensor share its counter
+        written = [t for p, g, c in zip(params, grads, self.copies) if g is not None for t in (p, c) if t is not None]
+        self._written = list({id(t): t for t in (t if t._base is None else t._base for t in written)}.values())
 
     @property
     def steps(self) -> torch.Tensor:
@@ -829,6 +832,9 @@ def adamw_multi(plan: AdamWPlan, lr, betas=(0.9, 0.99), eps: float = 1e-15, weig
         check(_lib.lib().hrf_adamw_multi(*plan._head, *plan._body, float(lr), ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
                                          float(weight_decay), float(grad_scale), 0.0 if max_norm is None else float(max_norm), ptr(norm),
                                          ptr(flags), ptr(scaler), plan.seed, 1 if zero_grad else 0, stream_of(plan.device.index)))
+    torch.autograd.graph.increment_version(plan._written)
+    if zero_grad and plan.grads is not None:
+        torch.autograd.graph.increment_version([g for g in plan.grads if g is not None])
 
 
 _INT8_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}

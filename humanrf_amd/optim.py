@@ -20,7 +20,7 @@ class AdamW(torch.optim.Optimizer):
     Gradients that stay in place from step to step (`zero_grad(set_to_none=False)`, or `step(zero_grad=True)`, which zeroes them in the
     same pass) cost nothing on the host; new ones are written into the descriptors first. A graph of the step is captured after one eager
     step with the gradients in place; its replays step the tensors that it was captured with, whatever gradients later eager steps are given.
-    `step` advances the parameters' version counters, so that casts of them are renewed."""
+    `step` advances the version counters of what it writes, so that casts of the parameters are renewed."""
 
     def __init__(self, params, lr=1e-2, betas=(0.9, 0.99), eps: float = 1e-15, weight_decay: float = 1e-2, state_bits: int = 32,
                  max_grad_norm: Optional[float] = None, seed: int = 0, copies: Optional[Dict[torch.Tensor, torch.Tensor]] = None):
@@ -110,7 +110,8 @@ class AdamW(torch.optim.Optimizer):
                         grad_scale=grad_scale, flags=flags, scaler=scaler, zero_grad=zero_grad)
         if torch.cuda.is_current_stream_capturing():
             plan._keep_captured(grads)
-        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+        if zero_grad:
+            torch.autograd.graph.increment_version(present)
         return loss
 
     # ------------------------------------------------------------------ checkpoints

@@ -329,3 +329,32 @@ def test_every_group_s_lr_and_decay_are_looked_at(host, bad):
     with pytest.raises(ValueError, match="finite and not negative"):
         opt.step()
     assert len(host.calls) == n
+
+
+def test_versions_of_what_a_step_writes(host):
+    """Through ops.adamw_multi as through the optimizer: a cast that is renewed by version (HumanRF's 16-bit copies) sees the step, and autograd
+    refuses to go back through what was overwritten."""
+    from humanrf_amd import ops
+    host.count = 2
+    p, q = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(5))
+    c, g = torch.zeros(4, dtype=torch.float16), torch.zeros(4)
+    plan = ops.AdamWPlan([p, q], [g, None], copies=[c, None])
+    watched = (p, q, c, g)
+    before = [t._version for t in watched]
+    ops.adamw_multi(plan, 1e-2)
+    assert [t._version - b for t, b in zip(watched, before)] == [1, 0, 1, 0]
+    ops.adamw_multi(plan, 1e-2, zero_grad=True)
+    assert [t._version - b for t, b in zip(watched, before)] == [2, 0, 2, 1]
+    x = torch.ones(4, requires_grad=True)
+    y = (x * c.float() * p).sum()
+    ops.adamw_multi(plan, 1e-2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    flat = torch.zeros(10)
+    views, version = [flat[:4], flat[4:]], flat._version
+    ops.adamw_multi(ops.AdamWPlan(views, [torch.ones(4), torch.ones(6)]), 1e-2)
+    assert flat._version == views[1]._version == version + 1
+    opt, (p,) = _stepped(host, [torch.zeros(4)])
+    before, g = (p._version, p.grad._version), p.grad
+    opt.step(zero_grad=True)
+    assert (p._version, g._version) == (before[0] + 1, before[1] + 1)
