@@ -611,11 +611,18 @@ def _on_device(device: torch.device):
     return _NOSPAN if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _disjoint(tensors, what: str) -> None:
-    """No two of the tensors share memory: workgroups step them side by side."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t is not None and t.numel() > 0)
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+def _spans(tensors) -> np.ndarray:
+    """(address, bytes) of each tensor that has a value."""
+    return np.array([(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t is not None and t.numel() > 0], dtype=np.int64).reshape(-1, 2)
+
+
+def _disjoint(what: str, *spans) -> np.ndarray:
+    """No two of the spans share memory: workgroups step them side by side."""
+    joined = np.concatenate(spans)
+    joined = joined[np.argsort(joined[:, 0], kind="stable")]
+    if (joined[:-1].sum(axis=1) > joined[1:, 0]).any():
         raise RuntimeError(f"AdamWPlan: two {what} share memory")
+    return joined
 
 
 _ADAMW_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -652,7 +659,7 @@ class AdamWPlan:
         copies = [None] * len(params) if copies is None else list(copies)
         if len(copies) != len(params):
             raise RuntimeError("AdamWPlan: one copy (or None) for each parameter")
-        self._check_params(params, copies, params[0].device)
+        spans = self._check_params(params, copies, params[0].device)
         self.params, self.copies, self.state_bits, self.seed = params, copies, int(state_bits), int(seed) & 0xFFFFFFFF
         self.device = params[0].device
         self.lr_scales = [1.0] * len(params) if lr_scales is None else [float(x) for x in lr_scales]
@@ -670,13 +677,14 @@ class AdamWPlan:
         self._rows = np.zeros(len(params), dtype=_ADAMW_TENSOR)
         self._rows["n"], self._rows["base"], self._rows["first_tile"] = lengths, self.offsets, np.cumsum(tiles) - tiles
         self.state = self._take_state(state)
+        self._state_spans = _spans(self.state.values())
         with _on_device(self.device):
             self._ctl = torch.zeros(_lib.ADAMW_CTL + len(params), dtype=torch.int32, device=self.device)
             if step:
                 self._ctl[_lib.ADAMW_CTL:] = int(step)
             self._ws = torch.empty(int(_lib.lib().hrf_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
         self.grads, self._desc, self._desc_captured, self._kept = None, None, False, []
-        self.set_grads([None] * len(params) if grads is None else grads)
+        self._point_at(params, spans, [None] * len(params) if grads is None else grads)
         # what the entry points take of the plan, as addresses: none of these buffers is ever replaced
         st = list(self.state.values())
         first, second, scales = (st[0], st[1], (None, None)) if self.state_bits == 32 else (st[0], st[2], (st[1], st[3]))
@@ -701,7 +709,7 @@ class AdamWPlan:
         return {name: state[name] for name in want}
 
     @staticmethod
-    def _check_params(params, copies, device) -> None:
+    def _check_params(params, copies, device) -> np.ndarray:
         for p in params:
             _chk(p, "parameter")
             if p.dtype not in _ADAMW_KINDS:
@@ -716,7 +724,7 @@ class AdamWPlan:
                 raise RuntimeError("AdamWPlan: copies are float16 or bfloat16 copies of float32 parameters")
             if c.numel() != p.numel() or c.device != p.device:
                 raise RuntimeError("AdamWPlan: a copy has its parameter's length and device")
-        _disjoint(params + copies, "parameters or copies")
+        return _disjoint("parameters or copies", _spans(params + copies))
 
     def set_tensors(self, params, grads) -> None:
         """Other storage for the parameters, each as long as the one it replaces (lengths, states and step counts are the plan's own), and
@@ -727,13 +735,12 @@ class AdamWPlan:
         for k, (p, n) in enumerate(zip(params, self._lengths)):
             if p.numel() != n:
                 raise RuntimeError(f"AdamWPlan: parameter {k} has {p.numel()} values, the plan was built over {n}: build another plan")
-        self._check_params(params, self.copies, self.device)
-        self._point_at(params, grads)
+        self._point_at(params, self._check_params(params, self.copies, self.device), grads)
 
     def set_grads(self, grads) -> None:
         """Other gradient tensors (or None) for the next steps: the descriptors are written anew, on the current stream. Replays of a
         graph that captured adamw_multi or grad_norm_multi read the same descriptors, so these are their gradients too."""
-        self._point_at(self.params, grads)
+        self._point_at(self.params, self._param_spans, grads)
 
     def _keep_captured(self, grads) -> None:
         """The step that was just captured goes on reading its descriptors and these gradients: they stay, and the next change of addresses
@@ -742,7 +749,7 @@ class AdamWPlan:
             self._kept.append((self._desc, self.params, list(grads)))
             self._desc_captured = True
 
-    def _point_at(self, params, grads) -> None:
+    def _point_at(self, params, spans, grads) -> None:
         grads = list(grads)
         if len(grads) != len(params):
             raise RuntimeError("AdamWPlan: one gradient (or None) for each parameter")
@@ -754,7 +761,7 @@ class AdamWPlan:
                 raise RuntimeError(f"AdamWPlan: gradients must be float32, float16 or bfloat16, got {g.dtype}")
             if g.numel() != n or g.device != self.device:
                 raise RuntimeError("AdamWPlan: a gradient has its parameter's length and device")
-        _disjoint(grads, "gradients")
+        _disjoint("parameters, copies, gradients or states", spans, self._state_spans, _spans(grads))
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWPlan: the gradients' addresses change inside the capture of a graph; keep them in place "
                                "(zero them instead of dropping them) and set them before the capture")
@@ -774,7 +781,7 @@ class AdamWPlan:
                 self._head = (ptr(self._desc), ptr(self._desc) + rows.nbytes, self.num_tiles)
             else:
                 self._desc[:rows.nbytes].copy_(torch.from_numpy(rows.view(np.uint8)).pin_memory(), non_blocking=True)
-        self.params, self.grads = params, grads
+        self.params, self.grads, self._param_spans = params, grads, spans
         # what a step writes, for autograd and for casts that are renewed by version; views of one tensor share its counter
         written = [t for p, g, c in zip(params, grads, self.copies) if g is not None for t in (p, c) if t is not None]
         self._written = list({id(t): t for t in (t if t._base is None else t._base for t in written)}.values())

@@ -531,7 +531,7 @@ int hrf_adam_multi(const hrf_adam_tensor* tensors, int count, int num_groups, in
  * the reference, whose optimizer is torch.optim.Adam on fp32 tensors (humanrf/run.py:101).
  * tensors: DEVICE array of `count` descriptors; tile_tensor: DEVICE int32[num_tiles], the tensor of each tile of 2048 elements, the
  * tiles of tensor k being first_tile .. first_tile + ceil(n / 2048) - 1.
- * No two tensors share memory, nor do two copies or two gradients.
+ * No two of the parameters, copies, gradients and states share memory.
  * States lie in flat buffers (at multiples of 16 bytes), tensor k's from position `base` (a multiple of 256) on, each tensor padded with zeros to whole blocks
  * of 256:
  *   state_bits 32: exp_avg, second = fp32 moments m and v;

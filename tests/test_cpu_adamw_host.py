@@ -358,3 +358,30 @@ def test_versions_of_what_a_step_writes(host):
     before, g = (p._version, p.grad._version), p.grad
     opt.step(zero_grad=True)
     assert (p._version, g._version) == (before[0] + 1, before[1] + 1)
+
+
+def test_nothing_that_a_step_writes_shares_memory(host):
+    """Workgroups work on the tensors side by side: a gradient inside another tensor's values, or values inside the states, would be read
+    before or after they are written."""
+    from humanrf_amd import ops
+    host.count = 2
+    buf, g = torch.zeros(2000), torch.zeros(2000)
+    p = [buf[:50], buf[50:100]]
+    plan = ops.AdamWPlan(p, [g[:50], g[50:100]])
+    for grads in ([buf[50:100], None], [buf[:50], None], [g[:50], g[49:99]]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            plan.set_grads(grads)
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.AdamWPlan(p, grads)
+    state = {"exp_avg": buf[64:576], "exp_avg_sq": g[200:712]}
+    with pytest.raises(RuntimeError, match="share memory|multiple of 16"):
+        ops.AdamWPlan(p, [g[:50], g[50:100]], state=state)
+    big = torch.zeros(4096)
+    at = (-big.data_ptr() // 4) % 4
+    whole = big[at:at + 1024]
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.AdamWPlan(p, state={"exp_avg": whole[:512], "exp_avg_sq": whole[256:768]})
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.AdamWPlan([whole[:50], whole[600:650]], state={"exp_avg": whole[:512], "exp_avg_sq": big[2048 + at:2560 + at]})
+    ops.AdamWPlan(p, [g[:50], g[50:100]], state={"exp_avg": whole[:512], "exp_avg_sq": whole[512:]})
+    assert np.array_equal(plan._rows["grad"], [g.data_ptr(), g.data_ptr() + 200])
