@@ -860,9 +860,10 @@ def _rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dim() < 1 or not 1 <= t.shape[-1] <= INT8_MAX_INNER:
         raise RuntimeError(f"{name}: 1 to {INT8_MAX_INNER} values a row, got shape {tuple(t.shape)}")
     if t.dim() != 2:
-        if not t.is_contiguous():
-            raise RuntimeError(f"Tensor not contiguous: {name}")
-        t = t.view(-1, t.shape[-1])
+        try:
+            t = t.view(-1, t.shape[-1])
+        except RuntimeError:
+            raise RuntimeError(f"Tensor not contiguous: {name} (its rows are not equally far apart)") from None
     if t.shape[0] > 0 and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         raise RuntimeError(f"Tensor not contiguous: {name} (within its rows)")
     return t

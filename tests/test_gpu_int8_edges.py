@@ -55,3 +55,29 @@ def test_packing_more_rows_than_an_axis_counts():
     for at in range(0, n // 16, 2 ** 22):
         part = p[at:at + 2 ** 22]
         assert int(part[:, :, 1:].ne(0).sum()) == 0 and int(part[:, 16:].ne(0).sum()) == 0
+
+
+# ------------------------------------------------------------------------------------------------ axes and strides
+@pytest.mark.parametrize("k", [33, 64, 130, 300])
+@pytest.mark.parametrize("lead", [(), (1,), (2, 3), (40, 5), (2, 0, 3)])
+def test_what_rounding_gives_is_what_the_product_takes(lead, k):
+    """Codes of x with any number of axes are rows further apart than they are long."""
+    from humanrf_amd import ops
+    h = ops.Int8Weight(_codes(20, k, 1), torch.rand(20, generator=_gen(2), device="cuda"))
+    x = torch.randn(*lead, k, generator=_gen(3), device="cuda")
+    q, s = ops.quantize_int8(x)
+    assert q.shape == x.shape and s.shape == x.shape[:-1]
+    y = ops.linear_int8(q, h, x_scale=s)
+    assert y.shape == (*lead, 20) and torch.equal(y, ops.linear_int8(x, h))
+
+
+def test_strides_that_are_no_rows_are_refused():
+    from humanrf_amd import ops
+    h = ops.Int8Weight(_codes(4, 32, 1), torch.ones(4, device="cuda"))
+    x = torch.zeros(6, 5, 32, device="cuda")
+    assert ops.linear_int8(x[:, ::5], h).shape == (6, 1, 4)
+    for bad in (x.transpose(0, 1), x[:, :3], x[:, :1].expand(6, 5, 32), torch.zeros(64, device="cuda")[::2], torch.zeros(2, 3, 64, device="cuda")[..., ::2]):
+        with pytest.raises(RuntimeError, match="not contiguous"):
+            ops.linear_int8(bad, h)
+        with pytest.raises(RuntimeError, match="not contiguous"):
+            ops.quantize_int8(bad)
