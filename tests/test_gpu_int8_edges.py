@@ -81,3 +81,38 @@ def test_strides_that_are_no_rows_are_refused():
             ops.linear_int8(bad, h)
         with pytest.raises(RuntimeError, match="not contiguous"):
             ops.quantize_int8(bad)
+
+
+# ------------------------------------------------------------------------------------------------ scales at the ends of fp32
+@pytest.mark.parametrize("m,n,k", [(1, 40, 300), (3, 40, 5000), (20, 70, 300), (60, 70, 300), (200, 300, 300), (300, 130, 2051), (2100, 2300, 1024), (700, 1100, 640),
+                                   (100, 70, 64), (100, 70, 128), (5000, 100, 200)])
+@pytest.mark.parametrize("token,channel", [(-125, -30), (-30, -125), (-80, -60), (-70, 100), (100, -70), (110, -126), (-149, 40), (40, -140), (-60, -60), (60, 60),
+                                           (-64, 64), (0, 0)])
+def test_products_of_scales_beyond_fp32(m, n, k, token, channel):
+    """sx sw may lie below or above what fp32 holds while sum sx sw does not: the same bound as for all other products, 3 U |v|, and half a
+    step of the smallest numbers, 2^-150, for the product and for the type each. Sums of zero stay zero where sx sw is beyond fp32."""
+    from humanrf_amd import ops
+    x, w = _codes(m, k, 1), _codes(n, k, 2)
+    x[m // 2] = 0
+    sx = torch.ldexp(torch.rand(m, generator=_gen(3), device="cuda") + 1.0, torch.tensor(token, device="cuda"))
+    sw = torch.ldexp(torch.rand(n, generator=_gen(4), device="cuda") + 1.0, torch.tensor(channel, device="cuda"))
+    y = ops.linear_int8(x, ops.Int8Weight(w, sw), x_scale=sx)
+    v = (x.double() @ w.double().t()) * sx.double()[:, None] * sw.double()
+    fits = v.abs() < 2.0 ** 127
+    assert bool(((y.double() - v).abs() <= 3 * U * v.abs() + 2.0 ** -149)[fits].all())
+    assert not bool(torch.isnan(y).any()) and int(y[m // 2].ne(0).sum()) == 0
+    big = ops.linear_int8(x, ops.Int8Weight(w, torch.full_like(sw, 2.0 ** 100)), x_scale=torch.full_like(sx, 2.0 ** 100))
+    assert not bool(torch.isnan(big).any()) and int(big[m // 2].ne(0).sum()) == 0 and torch.equal(torch.isinf(big), v != 0)
+
+
+@pytest.mark.parametrize("m,k", [(1, 300), (20, 300), (200, 300), (100, 64), (5000, 200)])
+def test_tiny_rows(m, k):
+    """Rows of 1e-34 against weights of 1e-3: products of 1e-36 in fp32, their scales' product below the normal numbers."""
+    from humanrf_amd import ops
+    x, w = torch.randn(m, k, generator=_gen(1), device="cuda") * 1e-34, torch.randn(70, k, generator=_gen(2), device="cuda") * 1e-3
+    q, s = ops.quantize_int8(x)
+    h = ops.Int8Weight.from_float(w)
+    v = (q.double() @ ops.quantize_int8(w)[0].double().t()) * s.double()[:, None] * h.scale.double()
+    y = ops.linear_int8(x, h)
+    assert bool(((y.double() - v).abs() <= 3 * U * v.abs() + 2.0 ** -149).all())
+    assert torch.equal(y, ops.linear_int8(q, h, x_scale=s))
