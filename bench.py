@@ -136,15 +136,22 @@ def parse():
     return ap.parse_args()
 
 
+# sources under csrc/ whose kernels no bench run launches
+OTHER_SOURCES = ("adamw.hip", "int8.hip")
+
+
 def kernel_source_fingerprint() -> str:
-    """SHA-256 over the kernel sources the library is built from (what a PMC summary under profiles/ is valid for)."""
+    """SHA-256 over the kernel sources that a bench run's kernels are built from and the flags they are built with (what a PMC summary
+    under profiles/ is valid for)."""
     import hashlib
     h = hashlib.sha256()
     d = os.path.join(ROOT, "humanrf_amd", "csrc")
     for name in sorted(os.listdir(d)):
-        if name.endswith((".hip", ".h", ".cpp")):
+        if name.endswith((".hip", ".h", ".cpp")) and name not in OTHER_SOURCES:
             h.update(name.encode())
             h.update(open(os.path.join(d, name), "rb").read())
+    make = open(os.path.join(d, "Makefile")).read()
+    h.update(make[make.index("FLAGS ="):make.index("SRCS =")].encode())
     return h.hexdigest()
 
 
@@ -692,7 +699,7 @@ def main():
                                                 "where": f"a window of {kw['steps']} steps behind the timed region"}
         # HBM-side traffic of the gather / scatter kernels comes from separate rocprofv3 --pmc passes (FETCH_SIZE, WRITE_SIZE,
         # TCC_ATOMIC: MI355X_MICROARCH.md) whose summary is committed with the fingerprint of the kernel sources it was taken
-        # on (tools/make_traffic_json.py); a summary taken on other sources is not reported.
+        # on (tools/pmc_summary.py); a summary taken on other sources is not reported.
         traffic_json, traffic_src = None, None
         fp = kernel_source_fingerprint()
         for name in sorted((f for f in os.listdir(os.path.join(ROOT, "profiles")) if f.endswith("_traffic.json")), reverse=True):

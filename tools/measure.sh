@@ -82,7 +82,7 @@ pmc)
   # HBM-side traffic (FETCH_SIZE, WRITE_SIZE) and memory-side atomic requests (TCC_ATOMIC_sum) of the gather / scatter kernels per
   # unit of work, and MfmaUtil of the MLP kernels: each counter in its own rocprofv3 pass (kernel trace + pmc only) over
   # tools/pmc_driver.py = the bench configuration ("$@": bench.py flags) after PM_WARM training steps. -> FETCH_SIZE.txt ...,
-  # traffic.json, mfma.json with the fingerprint of the kernel sources (copy to profiles/r06_traffic.json, profiles/r06_mfma.json:
+  # traffic.json, mfma.json with the fingerprint of the kernel sources (copy to profiles/training_step_traffic.json, _mfma.json:
   # bench.py reports them when the fingerprint matches the sources it runs).
   export PM_WARM=${PM_WARM:-1500}
   : > $L
