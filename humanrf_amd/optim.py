@@ -57,6 +57,10 @@ class AdamW(torch.optim.Optimizer):
             if any(g["lr"] is not first["lr"] for g in groups):
                 raise ValueError("AdamW: an lr that is a tensor is the same tensor in all parameter groups")
             lr, scale = first["lr"], [1.0] * len(groups)
+            if not lr.is_cuda:          # (a number for this call; one on the device is read there, by replays too)
+                lr = float(lr)
+                if not 0.0 <= lr < float("inf"):
+                    raise ValueError(f"AdamW: lr is finite and not negative, got {lr}")
         else:
             lr = max(float(g["lr"]) for g in groups)
             scale = [float(g["lr"]) / lr if lr > 0.0 else 1.0 for g in groups]

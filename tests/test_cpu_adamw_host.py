@@ -385,3 +385,18 @@ def test_nothing_that_a_step_writes_shares_memory(host):
         ops.AdamWPlan([whole[:50], whole[600:650]], state={"exp_avg": whole[:512], "exp_avg_sq": big[2048 + at:2560 + at]})
     ops.AdamWPlan(p, [g[:50], g[50:100]], state={"exp_avg": whole[:512], "exp_avg_sq": whole[512:]})
     assert np.array_equal(plan._rows["grad"], [g.data_ptr(), g.data_ptr() + 200])
+
+
+def test_an_lr_in_a_tensor_on_the_host_is_a_number(host):
+    """As torch.optim.AdamW takes it; a schedule writes into it."""
+    lr = torch.tensor(3e-3, dtype=torch.float64)
+    opt, params = _stepped(host, [torch.zeros(4), torch.zeros(7)], lr=lr)
+    assert host.calls[-1][1][10:12] == (3e-3, None)
+    lr.fill_(1e-3)
+    opt.step()
+    assert host.calls[-1][1][10:12] == (1e-3, None)
+    n = len(host.calls)
+    lr.fill_(-1.0)
+    with pytest.raises(ValueError, match="finite and not negative"):
+        opt.step()
+    assert len(host.calls) == n
