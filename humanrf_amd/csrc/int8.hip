@@ -263,13 +263,11 @@ __device__ __forceinline__ void i8_store(T* row, int n, int cols, bool here, con
 
 // 16 bytes from base + offset (each lane its own) to LDS, the wavefront's kilobyte from byte `to` on in the order of its lanes. The
 // compiler takes the builtin for this as something every later LDS read may depend on and waits for it at once; here the caller waits
-// (s_waitcnt vmcnt, a barrier) before anybody reads. m0 holds the address in LDS while the load is issued; it is reserved and
-// cannot be declared as written, so it is put back (8192^3: 520 us either way).
+// (s_waitcnt vmcnt, a barrier) before anybody reads. m0 holds the address in LDS; it is an input of the
+// statement, so that the compiler writes it and knows.
 __device__ __forceinline__ void i8_load_lds(const int8_t* base, uint32_t offset, uint32_t to)
 {
-    int kept;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(kept) : "s"(to), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(base) : "memory");
 }
 
 // Block -> tile: the blocks that run on one XCD (every eighth) take neighbouring tiles, in columns of 8 tiles of tokens, so that what they
