@@ -224,7 +224,12 @@ struct I8Args {
 // multiplied and the exponents put back at the end, so that nothing overflows or loses bits unless the result does. Both give the same bits
 // where the first is right; a workgroup takes the second way if one of its scales asks for it. Looking takes 0.4 us of 26 for
 // 1021 x 4099 x 2051 and 0.3 of 20.7 for 320000 x 64 x 64.
-__device__ __forceinline__ bool i8_is_wide(float scale) { return !(scale >= 0x1p-63f && scale <= 0x1p63f); }
+// 0, inf and NaN are not wide: both ways give the same.
+__device__ __forceinline__ bool i8_is_wide(float scale)
+{
+    const uint32_t bits = i8_bits(scale);
+    return bits - 1u < 0x1fffffffu || bits - 0x5f000001u < 0x207fffffu;
+}
 
 template <bool kWide>
 __device__ __forceinline__ float i8_scaled(int acc, float sx, float sw)
@@ -365,21 +370,10 @@ __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 8 ? 1 : 2) * WN / 2) void
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    bool odd = false;
-    for (int k = threadIdx.x; k < BM; k += kThreads) {
-        const float scale = A.sx[min(m0 + k, A.rows - 1)];
-        s_sx[k] = scale;
-        odd |= i8_is_wide(scale);
-    }
-    for (int k = threadIdx.x; k < BN; k += kThreads) {
-        const int n = min(n0 + k, A.cols - 1);
-        const float scale = A.sw[n];
-        s_sw[k] = scale;
-        odd |= i8_is_wide(scale);
-        s_bias[k] = A.bias ? A.bias[n] : 0.0f;
-    }
-    odd = __any(odd);
-    if (lane == 0) s_wide[wave] = odd;
+    // Scales and biases, a thread each, stay in registers until the products are done: nobody waits for them before the first stage.
+    static_assert(BM <= kThreads && BN <= kThreads, "a thread for each scale");
+    const int tx = min((int)threadIdx.x, BM - 1), tw = min((int)threadIdx.x, BN - 1), nw = min(n0 + tw, A.cols - 1);
+    const float scale_x = A.sx[min(m0 + tx, A.rows - 1)], scale_w = A.sw[nw], bias_w = A.bias ? A.bias[nw] : 0.0f;
 #pragma unroll
     for (int s = 0; s < 3; ++s)
 #pragma unroll
@@ -393,6 +387,12 @@ __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 8 ? 1 : 2) * WN / 2) void
         work(1, s + 1, 0, s + 3);       // (past the end: stages that are there, read again and not used)
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // nothing may land in LDS that is somebody else's by then
+    s_sx[tx] = scale_x;         // (of the threads past the end the last one's again)
+    s_sw[tw] = scale_w;
+    s_bias[tw] = bias_w;
+    const bool odd = __any(i8_is_wide(scale_x) || i8_is_wide(scale_w));
+    if (lane == 0) s_wide[wave] = odd;
+    __syncthreads();
 
     // Epilogue, 32 channels of 32 tokens at a time: a lane holds channels 8 g + 4 (lane / 32) + 0 .. 3 of token lane % 32. For 16-bit y the
     // halves of the wavefront trade, so that a lane has eight neighbouring channels, 16 bytes. (Through LDS, whole rows at a time, this
@@ -753,13 +753,31 @@ static bool i8_is_short(int64_t rows, int64_t cols, int64_t padded)
     return padded == 64 || (padded <= 256 && rows > 64 && (cols <= 192 || (cols <= 512 && rows <= 4096)));
 }
 
+// Workgroups of 256 threads of a kernel that the card holds at a time. The short rows' wavefronts walk over as many blocks each, so that
+// no round is left half empty: 300000 x 64 x 32 16.6 us against 18.3 with 2048 workgroups, 100000 x 128 x 128 18.4 against 22.0,
+// 100000 x 128 x 256 39.9 against 47.5.
+template <typename F>
+static int i8_resident(F kernel)
+{
+    int each = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, 256, 0) != hipSuccess || each < 1) each = 4;
+    return 256 * each;
+}
+
+template <int X, int K, int KS>
+static void i8_short_of(const I8Args& A, const I8Short& B, hipStream_t stream)
+{
+    static const int resident = i8_resident(k_linear_i8_short<X, K, KS>);
+    const dim3 grid((unsigned)std::min<int64_t>(((int64_t)A.rows + 63) / 64, resident), (unsigned)((A.cols + 63) / 64));
+    hipLaunchKernelGGL((k_linear_i8_short<X, K, KS>), grid, dim3(256), 0, stream, A, B);
+}
+
 template <int X, int K>
 static void i8_short(const I8Args& A, const I8Short& B, hipStream_t stream)
 {
-    const dim3 grid((unsigned)std::min<int64_t>(((int64_t)A.rows + 63) / 64, 2048), (unsigned)((A.cols + 63) / 64));
-    if (A.inner == 64) hipLaunchKernelGGL((k_linear_i8_short<X, K, 1>), grid, dim3(256), 0, stream, A, B);
-    else if (A.inner == 128) hipLaunchKernelGGL((k_linear_i8_short<X, K, 2>), grid, dim3(256), 0, stream, A, B);
-    else hipLaunchKernelGGL((k_linear_i8_short<X, K, 4>), grid, dim3(256), 0, stream, A, B);
+    if (A.inner == 64) i8_short_of<X, K, 1>(A, B, stream);
+    else if (A.inner == 128) i8_short_of<X, K, 2>(A, B, stream);
+    else i8_short_of<X, K, 4>(A, B, stream);
 }
 
 // Very few rows, by the time of the captured call against rounding in a launch before: 1 x 4096 x 4096 6.6 us against 8.4, 1 x 4096 x 14336
