@@ -12,9 +12,9 @@
 // parameter with a first moment never divides by eps alone.
 //
 // Both passes stream: 28 B a parameter with fp32 p, g, m, v, 16.06 B with 8-bit states. On MI355X, where a copy of 4 GiB reads and writes
-// 5.0 TB/s: 39 M fp32 parameters and their fp16 copy 191 us (6.1 TB/s) with 32-bit states, bound by HBM, and 131 us (5.4 TB/s) with 8-bit
-// ones, whose 88 vector instructions an element keep the vector unit busy three quarters of that time; the norm of 240 M fp32 gradients
-// 161 us (6.0 TB/s).
+// 5.0 TB/s: 39 M fp32 parameters and their fp16 copy 189 us (6.2 TB/s) with 32-bit states, bound by HBM, and 124 us (5.7 TB/s) with 8-bit
+// ones, whose 93 vector instructions an element keep the vector unit busy 78 % of that time; the norm of 240 M fp32 gradients 162 us
+// (5.9 TB/s).
 #include "hrf_common.h"
 #include <algorithm>
 #include <cmath>
@@ -124,7 +124,7 @@ __device__ __forceinline__ double aw_pow(double b, int32_t t)   // b^t by squari
 }
 
 // Square root and quotient from the hardware's approximations (1 ulp) and one step of Newton's method, whose remainder an fma gives
-// exactly: at most a few thousandths of an ulp over correct rounding, in 11 and 6 instructions where the library's take 18 and 11.
+// exactly: at most a few thousandths of an ulp over correct rounding, in 12 and 5 instructions where the library's take 18 and 11.
 // Root: below 2^-100 the value is taken times 2^64 (the approximation flushes what is not normal); 0, inf and NaN are their own roots: a
 // second moment beyond fp32 has no finite root, and the step that is divided by it is 0. Quotient: a denominator that is normal, inf or NaN.
 __device__ __forceinline__ float aw_sqrt(float x)
@@ -480,7 +480,7 @@ extern "C" int hrf_adamw_multi(const hrf_adamw_tensor* tensors, const int32_t* t
     // One tile per workgroup, so that the scheduler evens out the work: 39 M fp32 parameters with 32-bit states 191 us against 208 us with
     // 2048 workgroups striding over the tiles; 120 M bf16 ones 430 against 518. 8-bit states are near the vector unit's limit, and what a
     // workgroup computes once (the bias corrections, in fp64) counts: four neighbouring tiles each, where that leaves eight workgroups
-    // for every CU. 240 M parameters 698 us against 749 with one tile each, 39 M 134 against 146.
+    // for every CU. Calls timed by events: 240 M parameters 710 us against 738 with one tile each, 39 M 149 against 153.
     const int per = state_bits == 8 && num_tiles >= 4 * 2048 ? 4 : 1;
     const unsigned blocks = (unsigned)std::max(1, (num_tiles + per - 1) / per);    // (tensors without a value have a step count)
     if (state_bits == 32)

@@ -10,7 +10,7 @@
 // each, in which bytes 16 q .. 16 q + 15 of row t are the 16 bytes at 256 q + 16 t: what lane (t, q) of the first instruction takes. A
 // wavefront's load of an operand is then one kilobyte side by side. Few tokens are packed too; many stay rows, of which the tiles read 64
 // bytes at a time (rounding 8192 rows of 8192 straight into packed blocks takes 89 us, pieces of 16 bytes scattered by different
-// workgroups; into rows 32). 29 tokens x 10240 x 5120: both operands as rows, 16 pieces of 64 bytes a load, 31 us; packed 13.
+// workgroups; into rows 32 to 34). 29 tokens x 10240 x 5120: both operands as rows, 16 pieces of 64 bytes a load, 31 us; packed 13.
 // Epilogue in fp32, one rounding per operation, one to the type of y.
 #include "hrf_common.h"
 #include <algorithm>
@@ -63,7 +63,8 @@ __device__ __forceinline__ int64_t i8_at(int64_t row, int k, int64_t ld)
 }
 
 // kGroup lanes a row (a power of two up to a wavefront, or the whole workgroup of 256 joined through LDS). The row is read once, in 16-byte
-// pieces, and stays in registers, kPieces of them a lane. 8192 rows of 8192 bf16: 118 us read twice value by value, 32 us this way.
+// pieces, and stays in registers, kPieces of them a lane. 8192 rows of 8192 bf16: 118 us read twice value by value, 32 us this way
+// over and over on one input, 34 on six in turn, 40 to 47 between products.
 template <int K, bool kPacked, int kGroup, int kPieces>
 __global__ __launch_bounds__(256) void k_quantize_rows(const typename I8Type<K>::T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                             int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale)
@@ -293,12 +294,12 @@ __device__ __forceinline__ void i8_tile_of(int tiles_m, int tiles_n, int& tm, in
 // Everything is dealt out between the products: while the matrix cores work on 32 k, the operands of the next 32 are read from LDS and
 // a quarter of the loads of the third stage on is issued (sixteen loads in a row hold the wavefront up for as long as they take
 // to issue, half a stage). In the middle of a stage the workgroup meets: the next stage has landed, and nobody reads the one before.
-// 8192^3 with 256 x 256 tiles: 469 us (2.34 POP/s; the library's product of the same integers reaches 2.14), bound by power: the matrix
-// cores are at work 73 % of the clocks, of which the card makes 1.5 GHz under this load (random codes; with zeros a tenth less time). No
-// bank conflicts in LDS. Every 8192 k more take 417 us; the rest are the ends of the four tiles that each CU takes, where nothing is
+// 8192^3 with 256 x 256 tiles: 456 to 537 us from card to card and run to run (2.05 to 2.4 POP/s; the library's product of the same
+// integers reached 2.14 where this one took 469), bound by power: the matrix cores are at work 72 % of the clocks, of which the card makes
+// 1.4 to 1.5 GHz under this load (random codes; with zeros a tenth less time). No bank conflicts in LDS. Every 8192 k more take 417 us; the rest are the ends of the four tiles that each CU takes, where nothing is
 // multiplied. (Going from tile to tile in one workgroup, the next one's loads on their way meanwhile, took 505 us where one tile a
 // workgroup took 483: the registers for that are not there.) 8 wavefronts rather than 4 shorten the ends: 8192 x 8192 x 1024 109 us
-// against 119. 128 x 128 tiles are bound by what the L2 gives, some 13 TB/s.
+// against 119. 128 x 128 tiles read 8.6 GB for the same product in 640 us, 13 TB/s.
 template <int K, int TM, int TN, int WN, int R>
 __global__ __launch_bounds__(128 * WN, (TM * TN * WN > 8 ? 1 : 2) * WN / 2) void k_linear_i8(const I8Args A)
 {
@@ -746,7 +747,7 @@ static void i8_pack(const int8_t* x, int64_t rows, int64_t cols, int64_t ldx, in
 }
 
 // Rows of up to 256 values, where rounding them first (a launch, codes written and read again) costs more than reading x once for every 64
-// channels. Captured calls, this way against the other: 100000 x 64 x 128 15 us against 50, 100000 x 128 x 256 46 against 72, 100000 x 256 x 256
+// channels. Captured calls, this way against the other: 100000 x 64 x 128 15 us against 50, 100000 x 128 x 256 40 against 72, 100000 x 256 x 256
 // 81 against 63; 4000 x 128 x 128 4.4 against 6.0, 2000 x 512 x 128 4.7 against 6.1. Rows of up to 64 have no other way.
 static bool i8_is_short(int64_t rows, int64_t cols, int64_t padded)
 {
