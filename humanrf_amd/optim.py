@@ -15,7 +15,7 @@ class AdamW(torch.optim.Optimizer):
     """params, lr, betas, eps, weight_decay: as torch.optim.AdamW, with the reference's betas and eps as defaults; lr and weight_decay may
     differ between parameter groups, betas and eps may not. state_bits: 32 or 8 (ops.AdamWPlan). max_grad_norm: clip the gradients of all
     groups together to this norm; a step whose norm is not finite is then skipped. copies: {parameter: 16-bit tensor} refreshed by the
-    step. The parameters lie on one GPU.
+    step. The parameters lie on one GPU and keep their lengths: storage of another length is refused, of the same length taken over.
 
     Gradients that stay in place from step to step (`zero_grad(set_to_none=False)`, or `step(zero_grad=True)`, which zeroes them in the
     same pass) cost nothing on the host; new ones are written into the descriptors first. A graph of the step is captured after one eager

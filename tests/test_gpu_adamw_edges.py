@@ -190,3 +190,60 @@ def test_a_copy_of_the_optimizer_goes_on_as_the_original(bits):
     assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(ps, qs))
     assert all(torch.equal(v.float(), other._plan.state[n].float()) for n, v in opt._plan.state.items())
     assert other._plan.steps.tolist() == [4, 4]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replaced_storage_is_stepped_and_other_lengths_are_not(bits):
+    from humanrf_amd.optim import AdamW
+    ps, qs = _params((3000, 40), 7), _params((3000, 40), 7)
+    opt, twin = AdamW(ps, state_bits=bits), AdamW(qs, state_bits=bits)
+
+    def step(o, params, k):
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=_gen(k), device="cuda")
+        o.step()
+    for k in range(4):
+        step(opt, ps, k)
+        step(twin, qs, k)
+        ps[0].data = ps[0].data.clone()         # the same values somewhere else
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    held = ps[0].data
+    ps[0].grad = None
+    ps[0].data = held[:2999].clone()
+    ps[0].grad = torch.ones(2999, device="cuda")
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError, match="2999 values"):
+        opt.step()
+    assert all(torch.equal(p, b) for p, b in zip(ps, before)) and opt._plan.steps.tolist() == [4, 4]
+    ps[0].grad = None
+    ps[0].data = held
+    step(opt, ps, 9)
+    step(twin, qs, 9)
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_a_device_lr_and_a_captured_step_of_the_optimizer(keep):
+    """lr in one tensor on the device: replays read what a schedule wrote into it."""
+    from humanrf_amd.optim import AdamW
+    lr = torch.tensor([LR], device="cuda")
+    ps, qs = _params((500,), 8), _params((500,), 8)
+    opt, twin = AdamW(ps, lr=lr), AdamW(qs, lr=LR)
+    ps[0].grad, qs[0].grad = torch.ones(500, device="cuda"), torch.ones(500, device="cuda")
+    opt.step()
+    twin.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(zero_grad=not keep)
+    for k in range(3):
+        now = float(torch.tensor(LR / (k + 2)))
+        lr.fill_(now)
+        twin.param_groups[0]["lr"] = now
+        ps[0].grad.fill_(1.0 + k)
+        qs[0].grad.fill_(1.0 + k)
+        graph.replay()
+        twin.step(zero_grad=not keep)
+        torch.cuda.synchronize()
+        # (the first step had lr in fp32 here and in fp64 there; every step rounds the value once)
+        assert bool(((ps[0].double() - qs[0].double()).abs() <= 4 * U * (qs[0].double().abs() + LR)).all())
+        assert torch.equal(ps[0].grad, qs[0].grad)
